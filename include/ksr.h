@@ -752,6 +752,31 @@ int ksr_sm_experts_fwd(const float* x, int x_ld, int x_c0, const float* k, int k
                        const float* const* ptrs, const int* low, int n_experts, float* out, int B, int64_t HW,
                        ksr_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Group norm with an activation on channels-last tensors (host side: kan_sr/ops.py:group_norm_act).  No counterpart in the
+ * reference, whose networks normalise with BatchNorm2d.
+ *   xhat = (x - mean) / sqrt(var + eps) over the S * C / G values of (image, group), var the biased variance;
+ *   y = act(weight[c] * xhat + bias[c])
+ * x (and dy) [B, S, C] with the channels contiguous and pixels / images the given numbers of ELEMENTS apart (a channel slice
+ * of a wider tensor is read in place; any alignment), fp32, or bf16 with bf16 != 0; y, dx dense in the same type.  weight, bias
+ * [C] fp32, NULL = ones / zeros.  stats [B][G][2] = mean, 1 / sqrt(var + eps): written by the forward, read by the backward.
+ * All arithmetic and sums are fp32, y and dx are rounded once; sums have a fixed order (results are the same from run to
+ * run).  The backward writes what is not NULL of dx, dweight, dbias.  ws: ksr_group_norm_ws_floats floats, free again when
+ * the call's kernels have run; every call that may overlap another needs its own.  B or S may be 0.
+ * ------------------------------------------------------------------------------------------- */
+#define KSR_ACT_NONE 0
+#define KSR_ACT_RELU 1
+#define KSR_ACT_SILU 2   /* z / (1 + exp(-z)) */
+#define KSR_ACT_GELU 3   /* z (1 + erf(z / sqrt 2)) / 2 */
+int64_t ksr_group_norm_ws_floats(int64_t B, int64_t S, int C, int G, int backward);   /* negative: refused, see ksr_last_error */
+int ksr_group_norm_fwd(const void* x, int64_t x_image_stride, int64_t x_pixel_stride, const float* weight, const float* bias,
+                       void* y, float* stats, float* ws, int64_t B, int64_t S, int C, int G, float eps, int act, int bf16,
+                       ksr_stream_t stream);
+int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t x_pixel_stride, const void* dy, int64_t dy_image_stride,
+                       int64_t dy_pixel_stride, const float* weight, const float* bias, const float* stats, void* dx,
+                       float* dweight, float* dbias, float* ws, int64_t B, int64_t S, int C, int G, int act, int bf16,
+                       ksr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from contextlib import nullcontext
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p, POINTER
 
 import torch
@@ -81,6 +82,7 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ksr_fused_wgrad_slab_floats.restype = c_int64
     L.ksr_in_proj_bwd_wg_slab_floats.restype = c_int64
     L.ksr_tx_bwd_wg_slab_floats.restype = c_int64
+    L.ksr_group_norm_ws_floats.restype = c_int64
 
 
 # every symbol include/ksr.h declares (tests/test_host_logic.py compares the two lists)
@@ -108,6 +110,7 @@ EXPORTS = [
     "ksr_unet_wgrad_slab_floats", "ksr_unet_wgrad", "ksr_unet_bn_bwd_partials", "ksr_unet_bn_relu_bwd", "ksr_unet_grad_merge",
     "ksr_unet_s2_dgrad", "ksr_unet_att_mix_bwd", "ksr_gather_batch",
     "ksr_kan_lin_slab_floats", "ksr_kan_lin_fwd", "ksr_kan_lin_bwd",
+    "ksr_group_norm_ws_floats", "ksr_group_norm_fwd", "ksr_group_norm_bwd",
 ]
 
 
@@ -141,6 +144,13 @@ def stream() -> c_void_p:
     if _RAW_STREAM is not None and _RAW_DEVICE is not None:
         return c_void_p(_RAW_STREAM(_RAW_DEVICE()))
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which t's device is the current one (stream() and the launches follow the current device)."""
+    if _RAW_DEVICE is not None and _RAW_DEVICE() == t.device.index:
+        return nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def host_floats(values) -> ctypes.Array:

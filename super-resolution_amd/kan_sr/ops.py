@@ -5,13 +5,13 @@ forward and backward below is one or more hand-written HIP kernels.
 """
 from __future__ import annotations
 
-from ctypes import c_int, c_int64
-from typing import Sequence
+from ctypes import c_float, c_int, c_int64, c_void_p
+from typing import Optional, Sequence
 
 import torch
 
 from . import _lib
-from ._lib import check, host_floats, lib, ptr, stream
+from ._lib import KsrError, check, host_floats, lib, on_device_of, ptr, stream
 
 
 def make_knots(grid_size: int, spline_order: int, grid_range: Sequence[float]) -> list:
@@ -186,3 +186,102 @@ def bilinear_up_into(x: torch.Tensor, out: torch.Tensor, r: int, in_channel0: in
                                 c_int64(C * H * W), c_int(in_channel0), c_int64(out.shape[1] * H * r * W * r),
                                 c_int(out_channel0), stream()),
           "ksr_bilinear_up")
+
+
+# ------------------------------------------------------------------------------------------------ group norm + activation
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}          # KSR_ACT_* of include/ksr.h
+
+
+def _pixel_rows(t: torch.Tensor):
+    """t [B, ..., C] -> (t or a dense copy, image stride, pixel stride, pixels): in place where the channels are contiguous
+    and the middle dimensions are one run of pixels (dense tensors, channel slices, images of a larger buffer)."""
+    B, C, mid = t.shape[0], t.shape[-1], list(zip(t.shape[1:-1], t.stride()[1:-1]))
+    S = 1
+    for n, _ in mid:
+        S *= n
+    if t.numel() == 0:
+        return t, 0, 0, S
+    run, step = 1, None                          # pixels in the run so far, its pixel stride
+    fits = C == 1 or t.stride(-1) == 1
+    for n, st in reversed(mid):
+        if n == 1:
+            continue
+        if step is None:
+            step = st
+        fits = fits and st == step * run
+        run *= n
+    if not fits:
+        t = t.contiguous()
+        return t, S * C, C, S
+    return t, t.stride(0) if B > 1 else 0, step if step is not None else 0, S
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        x, xb, xp, S = _pixel_rows(x)
+        B, C = x.shape[0], x.shape[-1]
+        bf16 = x.dtype is torch.bfloat16
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        stats = torch.empty(B, groups, 2, device=x.device, dtype=torch.float32)
+        with on_device_of(x):
+            n = int(lib().ksr_group_norm_ws_floats(c_int64(B), c_int64(S), c_int(C), c_int(groups), c_int(0)))
+            check(min(n, 0), "ksr_group_norm_ws_floats")
+            ws = torch.empty(n, device=x.device, dtype=torch.float32)
+            check(lib().ksr_group_norm_fwd(c_void_p(x.data_ptr()), c_int64(xb), c_int64(xp), ptr(weight), ptr(bias), ptr(y),
+                                           ptr(stats), ptr(ws), c_int64(B), c_int64(S), c_int(C), c_int(groups), c_float(eps),
+                                           c_int(act), c_int(bf16), stream()), "ksr_group_norm_fwd")
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.cfg = (groups, act, xb, xp, S)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        groups, act, xb, xp, S = ctx.cfg
+        B, C = x.shape[0], x.shape[-1]
+        dy, db_, dp, _ = _pixel_rows(dy)
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_x else None
+        dw = torch.empty(C, device=x.device, dtype=torch.float32) if want_w else None
+        db = torch.empty(C, device=x.device, dtype=torch.float32) if want_b else None
+        with on_device_of(x):
+            n = int(lib().ksr_group_norm_ws_floats(c_int64(B), c_int64(S), c_int(C), c_int(groups), c_int(1)))
+            check(min(n, 0), "ksr_group_norm_ws_floats")
+            ws = torch.empty(n, device=x.device, dtype=torch.float32)
+            check(lib().ksr_group_norm_bwd(c_void_p(x.data_ptr()), c_int64(xb), c_int64(xp), c_void_p(dy.data_ptr()),
+                                           c_int64(db_), c_int64(dp), ptr(weight), ptr(bias), ptr(stats), ptr(dx), ptr(dw), ptr(db),
+                                           ptr(ws), c_int64(B), c_int64(S), c_int(C), c_int(groups), c_int(act),
+                                           c_int(x.dtype is torch.bfloat16), stream()), "ksr_group_norm_bwd")
+        return dx, dw, db, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, eps: float = 1e-5, activation: str = "none") -> torch.Tensor:
+    """act(GroupNorm(x)) of a channels-last tensor x [B, ..., C], differentiable with respect to x, weight and bias.
+
+    The C channels form num_groups groups of neighbouring channels; mean and biased variance are taken over the pixels
+    and channels of a group of one image.  activation: "none", "relu", "silu" or "gelu" (the exact one).  x float32 or
+    bfloat16, weight and bias [C] float32 or None; statistics and sums are fp32, the result has x's type and is dense.
+    A channel slice of a wider tensor is read in place; of an NCHW tensor in torch.channels_last layout pass
+    x.permute(0, 2, 3, 1)."""
+    if activation not in ACTIVATIONS:
+        raise KsrError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    if x.dim() < 2:
+        raise KsrError(f"group_norm_act: x must be [B, ..., C], got {tuple(x.shape)}")
+    if not x.is_cuda:
+        raise KsrError("libksr ops need GPU tensors (the HIP path is the only path)")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise KsrError(f"group_norm_act: x must be float32 or bfloat16, got {x.dtype}")
+    C = x.shape[-1]
+    if num_groups < 1 or C < 1 or C % num_groups:
+        raise KsrError(f"group_norm_act: {C} channels do not form {num_groups} groups")
+    if not eps >= 0:
+        raise KsrError(f"group_norm_act: eps = {eps}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != (C,) or t.dtype is not torch.float32 or t.device != x.device):
+            raise KsrError(f"group_norm_act: {name} must be float32 [{C}] on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    return _GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation])
