@@ -777,6 +777,32 @@ int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t x_pixel_st
                        float* dweight, float* dbias, float* ws, int64_t B, int64_t S, int C, int G, int act, int bf16,
                        ksr_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Orthogonalisation by Newton-Schulz products and the Muon update (host side: kan_sr/muon.py).  No counterpart in the
+ * reference, which trains with Adam.  For every matrix U [rows, cols] (transposed in between where rows > cols):
+ *   X = U / (|U|_F + eps);   steps times:  A = X X^T,  X = a X + (b A + c A A) X
+ * muon = 0: U = src, dst = X (dense [batch][rows][cols], type of src: fp32, or bf16 with bf16 != 0);
+ * muon = 1 (fp32): g = grad_scale * src, momentum = momentum_factor * momentum + g, U = g + momentum_factor * momentum
+ *   (nesterov) or momentum;  dst = (1 - lr weight_decay) dst - lr scale sqrt(max(rows, cols)) X.  momentum, dst dense.
+ * split != 0: products of f16 pairs (22 bits), as close to 64 bits as fp32 arithmetic; 0: single f16 operands (diagonals and
+ *   the linear term apart), about 1e-3 off, for bf16 results.
+ * mats: HOST array, read during the call.  src may have any non-negative element strides; src and dst may be the same memory.
+ * The matrices of one call must not overlap in dst and momentum.  lr_dev: NULL, or a device float that replaces lr (recorded
+ * graphs).  ws: ksr_muon_ws_bytes bytes of device memory, 16-byte aligned, free again when the call's kernels have run; calls
+ * that may overlap need one each.  A matrix with a non-finite element becomes NaN throughout.  Refused: coefficients with
+ * which a singular value, or an eigenvalue of A or b A + c A A, could pass 30 within the steps. */
+typedef struct {
+    const void* src;
+    void* dst;
+    float* momentum;                               /* NULL with muon = 0 */
+    int64_t row_stride, col_stride, batch_stride;  /* of src, in elements */
+    int32_t rows, cols, batch, reserved;
+} KsrMatrix;
+int64_t ksr_muon_ws_bytes(const KsrMatrix* mats, int count, int split);       /* negative: refused, see ksr_last_error */
+int ksr_muon_batch(const KsrMatrix* mats, int count, int bf16, int split, int muon, int steps, float a, float b, float c,
+                   float eps, float momentum_factor, int nesterov, float grad_scale, float lr, const float* lr_dev,
+                   float weight_decay, float scale, void* ws, int64_t ws_bytes, ksr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,6 +83,7 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ksr_in_proj_bwd_wg_slab_floats.restype = c_int64
     L.ksr_tx_bwd_wg_slab_floats.restype = c_int64
     L.ksr_group_norm_ws_floats.restype = c_int64
+    L.ksr_muon_ws_bytes.restype = c_int64
 
 
 # every symbol include/ksr.h declares (tests/test_host_logic.py compares the two lists)
@@ -110,7 +111,7 @@ EXPORTS = [
     "ksr_unet_wgrad_slab_floats", "ksr_unet_wgrad", "ksr_unet_bn_bwd_partials", "ksr_unet_bn_relu_bwd", "ksr_unet_grad_merge",
     "ksr_unet_s2_dgrad", "ksr_unet_att_mix_bwd", "ksr_gather_batch",
     "ksr_kan_lin_slab_floats", "ksr_kan_lin_fwd", "ksr_kan_lin_bwd",
-    "ksr_group_norm_ws_floats", "ksr_group_norm_fwd", "ksr_group_norm_bwd",
+    "ksr_group_norm_ws_floats", "ksr_group_norm_fwd", "ksr_group_norm_bwd", "ksr_muon_ws_bytes", "ksr_muon_batch",
 ]
 
 

@@ -1,0 +1,183 @@
+"""Newton-Schulz orthogonalisation of matrices and the Muon optimiser on the HIP path.
+
+Muon replaces a weight matrix's momentum by the nearest (semi-)orthogonal matrix, approximately: with X = U / |U|_F a few
+steps of X <- a X + (b A + c A A) X, A = X X^T, drive every singular value towards 1.  The products, the momentum update before
+them and the weight update after them are kernels of libksr (ksr_muon_batch); matrices with a shorter side of up to 64, which
+is all this package's hyper-encoders have, run in one launch for the whole list.
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import byref, c_float, c_int, c_int32, c_int64, c_void_p
+from typing import Iterable, Optional, Sequence
+
+import torch
+
+from ._lib import KsrError, check, lib, on_device_of, stream
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+class _Matrix(ctypes.Structure):                  # KsrMatrix of include/ksr.h
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("momentum", c_void_p), ("row_stride", c_int64), ("col_stride", c_int64),
+                ("batch_stride", c_int64), ("rows", c_int32), ("cols", c_int32), ("batch", c_int32), ("reserved", c_int32)]
+
+
+def _run(mats, device_of: torch.Tensor, bf16: bool, split: bool, steps: int, coefficients, eps: float, muon: bool = False,
+         momentum: float = 0.0, nesterov: bool = False, grad_scale: float = 1.0, lr: float = 0.0,
+         lr_dev: Optional[torch.Tensor] = None, weight_decay: float = 0.0, scale: float = 0.0) -> None:
+    L = lib()
+    n = c_int(len(mats))
+    with on_device_of(device_of):
+        nbytes = int(L.ksr_muon_ws_bytes(mats, n, c_int(split)))
+        check(min(nbytes, 0), "ksr_muon_ws_bytes")
+        ws = torch.empty(nbytes, device=device_of.device, dtype=torch.uint8) if nbytes else None
+        a, b, c = coefficients
+        check(L.ksr_muon_batch(mats, n, c_int(bf16), c_int(split), c_int(muon), c_int(steps), c_float(a), c_float(b), c_float(c),
+                               c_float(eps), c_float(momentum), c_int(nesterov), c_float(grad_scale), c_float(lr),
+                               c_void_p(lr_dev.data_ptr() if lr_dev is not None else 0), c_float(weight_decay), c_float(scale),
+                               c_void_p(ws.data_ptr() if nbytes else 0), c_int64(nbytes), stream()), "ksr_muon_batch")
+
+
+def _steps_and_coefficients(steps, coefficients):
+    if not 1 <= int(steps) <= 32:
+        raise KsrError(f"newton_schulz: {steps} steps (1 to 32)")
+    if len(coefficients) != 3:
+        raise KsrError(f"newton_schulz: three coefficients (a, b, c), got {coefficients!r}")
+    return int(steps), tuple(float(v) for v in coefficients)
+
+
+def _split(precision: Optional[str], dtype: torch.dtype) -> bool:
+    if precision not in (None, "fp32", "bf16"):
+        raise KsrError(f"precision must be 'fp32' or 'bf16', got {precision!r}")
+    return dtype is torch.float32 if precision is None else precision == "fp32"
+
+
+def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7,
+                  precision: Optional[str] = None) -> torch.Tensor:
+    """Orthogonalises the matrices g [..., rows, cols] (float32 or bfloat16, any strides): a dense tensor of g's shape and type.
+
+    X = g / (|g|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (of the transposed matrix where
+    rows > cols).  precision: "fp32" (default for float32) forms the products to fp32 accuracy, "bf16" (default for bfloat16) to
+    that of a bfloat16 result at a third of the matrix work.  Not differentiable."""
+    steps, coefficients = _steps_and_coefficients(steps, coefficients)
+    if g.dim() < 2:
+        raise KsrError(f"newton_schulz: g must be [..., rows, cols], got {tuple(g.shape)}")
+    if not g.is_cuda:
+        raise KsrError("libksr ops need GPU tensors (the HIP path is the only path)")
+    if g.dtype not in (torch.float32, torch.bfloat16):
+        raise KsrError(f"newton_schulz: g must be float32 or bfloat16, got {g.dtype}")
+    if g.requires_grad and torch.is_grad_enabled():
+        raise KsrError("newton_schulz is not differentiable: detach g")
+    split = _split(precision, g.dtype)
+    out = torch.empty(g.shape, device=g.device, dtype=g.dtype)
+    if g.numel() == 0:
+        return out
+    u = g.detach()
+    u = u.unsqueeze(0) if u.dim() == 2 else u.reshape(-1, *u.shape[-2:])
+    if max(u.shape) > 1 << 24:
+        raise KsrError(f"newton_schulz: {tuple(g.shape)} is too large")
+    mats = (_Matrix * 1)()
+    mats[0] = (u.data_ptr(), out.data_ptr(), None, u.stride(1), u.stride(2), u.stride(0), u.shape[1], u.shape[2], u.shape[0], 0)
+    _run(mats, g, g.dtype is torch.bfloat16, split, steps, coefficients, eps)
+    return out
+
+
+def as_matrix(shape: Sequence[int]):
+    """(rows, cols) of a parameter: the first dimension against all others, so a convolution's [out, in, kh, kw] is
+    [out, in * kh * kw].  None for vectors and scalars, which Muon does not take."""
+    if len(shape) < 2:
+        return None
+    cols = 1
+    for n in shape[1:]:
+        cols *= n
+    return shape[0], cols
+
+
+def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+                steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7, scale: float = 0.2,
+                grad_scale: float = 1.0, precision: Optional[str] = None, lr_dev: Optional[torch.Tensor] = None) -> None:
+    """One Muon update of a list of float32 GPU tensors, in place, in few launches:
+
+        m <- momentum m + grad_scale g;   U = grad_scale g + momentum m (nesterov) or m;   O = newton_schulz(U)
+        w <- (1 - lr weight_decay) w - lr scale sqrt(max(rows, cols)) O
+
+    scale = 0.2 gives an update the root mean square of a typical Adam step, so that one learning rate serves both.  lr_dev: a
+    one-element float32 GPU tensor that replaces lr (recorded graphs)."""
+    steps, coefficients = _steps_and_coefficients(steps, coefficients)
+    weights, grads, momenta = list(weights), list(grads), list(momenta)
+    if not len(weights) == len(grads) == len(momenta):
+        raise KsrError(f"muon_update: {len(weights)} weights, {len(grads)} gradients, {len(momenta)} momenta")
+    if not weights:
+        return
+    device = weights[0].device
+    if device.type != "cuda":
+        raise KsrError("libksr ops need GPU tensors (the HIP path is the only path)")
+    f32 = torch.float32
+    if lr_dev is not None and (lr_dev.dtype is not f32 or lr_dev.numel() != 1 or lr_dev.device != device):
+        raise KsrError("muon_update: lr_dev must be one float32 on the weights' device")
+    mats = (_Matrix * len(weights))()
+    held, seen = [], set()
+    for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
+        shape = as_matrix(w.shape)
+        if shape is None:
+            raise KsrError(f"muon_update: tensor {i} is {tuple(w.shape)}: matrices only (vectors belong to Adam)")
+        if max(shape) > 1 << 24:
+            raise KsrError(f"muon_update: tensor {i}: {tuple(w.shape)} is too large")
+        if not (w.dtype is g.dtype is m.dtype is f32) or w.device != device or g.device != device or m.device != device:
+            raise KsrError(f"muon_update: tensor {i}: weight, gradient and momentum must be float32 on {device}")
+        if g.shape != w.shape or m.shape != w.shape or not w.is_contiguous() or not m.is_contiguous():
+            raise KsrError(f"muon_update: tensor {i}: gradient and momentum must have the weight's shape {tuple(w.shape)}, weight "
+                           "and momentum be contiguous")
+        if g.dim() > 2 or g.layout is not torch.strided:
+            g = g.contiguous().view(shape)
+            held.append(g)
+        wp, mp = w.data_ptr(), m.data_ptr()
+        if w.numel() and (wp in seen or mp in seen or wp == mp):
+            raise KsrError(f"muon_update: tensor {i}'s weight or momentum is in the list twice")
+        seen.update((wp, mp))
+        mats[i] = (g.data_ptr(), wp, mp, g.stride(0), g.stride(1), 0, shape[0], shape[1], 1, 0)
+    _run(mats, weights[0], False, _split(precision, f32), steps, coefficients, eps, True, momentum, nesterov, grad_scale, lr,
+         lr_dev, weight_decay, scale)
+    # the kernels write behind torch's back: whoever keys on the version counters (autograd, the UNet's kernel-layout weights) sees it
+    torch.autograd.graph.increment_version(weights + momenta)
+
+
+class Muon(torch.optim.Optimizer):
+    """torch optimiser over muon_update for parameters of two or more dimensions (convolutions as [out, in * kh * kw]);
+    vectors (biases, norms) belong to another optimiser.  Keeps one fp32 momentum per parameter (state "momentum_buffer")."""
+
+    def __init__(self, params: Iterable, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7,
+                 scale: float = 0.2, precision: Optional[str] = None):
+        steps, coefficients = _steps_and_coefficients(steps, coefficients)
+        if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1 or eps < 0:
+            raise KsrError(f"Muon: lr = {lr}, momentum = {momentum}, weight_decay = {weight_decay}, eps = {eps}")
+        _split(precision, torch.float32)
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=coefficients, eps=eps, scale=scale, precision=precision))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() < 2 or p.dtype is not torch.float32:
+                    raise KsrError(f"Muon takes float32 parameters of two or more dimensions, got {p.dtype} {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            weights, grads, momenta = [], [], []
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if "momentum_buffer" not in state:
+                    state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                weights.append(p)
+                grads.append(p.grad)
+                momenta.append(state["momentum_buffer"])
+            muon_update(weights, grads, momenta, group["lr"], group["momentum"], group["nesterov"], group["weight_decay"],
+                        group["steps"], group["coefficients"], group["eps"], group["scale"], precision=group["precision"])
+        return loss

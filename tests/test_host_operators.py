@@ -55,3 +55,47 @@ def test_pixel_rows(shape, stride, want):
         assert u.is_contiguous() and (ib, ip) == (n * shape[-1], shape[-1])
     else:
         assert (ib, ip) == want and u.data_ptr() == t.data_ptr()
+
+
+def test_muon_refuses_what_it_cannot_take():
+    from kan_sr._lib import KsrError
+    from kan_sr.muon import Muon, as_matrix, muon_update, newton_schulz
+    w = torch.randn(4, 4)
+    for bad in (lambda: newton_schulz(w), lambda: newton_schulz(w, steps=0), lambda: newton_schulz(w, coefficients=(1.0, 2.0)),
+                lambda: muon_update([w], [w], [w.clone()], lr=0.1), lambda: Muon([torch.nn.Parameter(w[0])]),
+                lambda: Muon([torch.nn.Parameter(w.double())]), lambda: Muon([torch.nn.Parameter(w)], momentum=1.0),
+                lambda: Muon([torch.nn.Parameter(w)], precision="fp64")):
+        with pytest.raises(KsrError):
+            bad()
+    assert as_matrix((64, 32, 3, 3)) == (64, 288) and as_matrix((5,)) is None and as_matrix((5, 7)) == (5, 7)
+
+
+def test_muon_refuses_at_the_abi():
+    from kan_sr import _lib
+    from kan_sr.muon import _Matrix
+    L = _lib.lib()
+    A = 1 << 20                                  # addresses that are never read: the checks come first
+
+    def one(src=A, dst=A, mom=A, rs=8, rows=8, cols=8, batch=1):
+        m = (_Matrix * 1)()
+        m[0] = (src, dst, mom, rs, 1, 0, rows, cols, batch, 0)
+        return m
+
+    def call(mats, bf16=0, muon=1, steps=5, coef=(3.4445, -4.775, 2.0315), eps=1e-7, ws=None, ws_bytes=0, count=1):
+        return L.ksr_muon_batch(mats, c_int(count), c_int(bf16), c_int(1), c_int(muon), c_int(steps), *(c_float(v) for v in coef),
+                                c_float(eps), c_float(0.9), c_int(1), c_float(1.0), c_float(0.1), None, c_float(0.0), c_float(0.2),
+                                ws, c_int64(ws_bytes), None)
+
+    assert call(one(src=None)) == -1 and call(one(dst=None)) == -1 and call(one(mom=None)) == -1
+    assert b"null pointer" in L.ksr_last_error()
+    assert call(None) == -1 and call(one(rows=-1)) == -1 and call(one(rs=-8)) == -1 and call(one(src=A + 2)) == -1
+    assert call(one(), bf16=1) == -1 and call(one(), steps=0) == -1 and call(one(), steps=33) == -1
+    assert call(one(), eps=float("nan")) == -1 and call(one(), eps=float("inf")) == -1
+    assert call(one(), coef=(9.0, 0.0, 0.0)) == -2 and b"coefficients" in L.ksr_last_error()
+    assert call(one(), coef=(float("nan"), 0.0, 0.0)) == -2
+    assert call(one(rows=1 << 21)) == -2 and call(one(rows=1 << 16, cols=1 << 16)) == -2 and call(one(batch=1 << 25)) == -2
+    assert call(one(rows=100, cols=100)) == -1 and b"workspace" in L.ksr_last_error()
+    need = L.ksr_muon_ws_bytes(one(rows=100, cols=100), c_int(1), c_int(1))
+    assert need > 0 and L.ksr_muon_ws_bytes(one(rows=64, cols=1024), c_int(1), c_int(1)) == 0
+    assert call(one(rows=100, cols=100), ws=c_void_p(A + 8), ws_bytes=need) == -1
+    assert call(one(rows=0)) == 0 and call(None, count=0) == 0
