@@ -579,6 +579,13 @@ int ksr_adam_step_dev(float* params, const float* grads, float* exp_avg, float* 
                       const float* lr_dev, float beta1, float beta2, float eps, float weight_decay,
                       const uint64_t* step_dev, float grad_scale, ksr_stream_t stream);
 
+/* Either form over parts of the flat buffers: runs is a HOST array of n_runs (first, length) pairs.  lr_dev and step_dev
+ * (both or neither) replace lr and step as in ksr_adam_step_dev.  The rest of the buffers is not touched (the parameters that
+ * ksr_muon_batch updates). */
+int ksr_adam_step_runs(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, const int64_t* runs, int n_runs,
+                       float lr, const float* lr_dev, float beta1, float beta2, float eps, float weight_decay, int step,
+                       const uint64_t* step_dev, float grad_scale, ksr_stream_t stream);
+
 /* Dropout stream id from device memory, for the same reason: while the CALLING THREAD has a device word set here, every
  * entry point with a (p_drop, seed) pair draws its masks from seed + word * 0x9E3779B97F4A7C15 (the word is read when
  * the kernel executes); the forward and backward entry points of one step must see the same word.  NULL (the default)

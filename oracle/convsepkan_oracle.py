@@ -273,19 +273,20 @@ def ycbcr_to_rgb(image: torch.Tensor) -> torch.Tensor:
 def conv_sep_kan_forward(x: torch.Tensor, p: Params, *, out_channels: Sequence[int],
                          grid_size: int, spline_order: int, grid_range: Sequence[float],
                          upscale: int, in_channels: Sequence[int] = (1,), attention: bool = False,
-                         backbone: str = "gazetr", train: bool = False, stats: Optional[dict] = None) -> torch.Tensor:
+                         backbone: str = "gazetr", train: bool = False, stats: Optional[dict] = None,
+                         norm_groups: int = 0) -> torch.Tensor:
     """x [B,3,H,W] (Y,Cb,Cr) -> [B,3,rH,rW].  Every layer sees the Y plane; only the
     last layer's output survives (the reference's loop overwrites y).
     attention=True: the `feed` 1x1 conv is replaced by chan_attention (parameters under `...feed.`), a wiring
     the reference itself does not contain (its ConvSepKanAttention is a stand-alone module).
     backbone="unet": the hyper-encoder is `unet` (conv_sep_kan_encoder.py:7,17 with UNet in place of GazeTR); `train`
-    and `stats` are its BatchNorm mode and running-statistics output."""
+    and `stats` are its BatchNorm mode and running-statistics output; norm_groups > 0: its GroupNorm form."""
     n_layers = len(out_channels)
     li = n_layers - 1
     prefix = f"layers.{li}.encoder.encoder."
     yplane = x[:, :1]
     if backbone == "unet":
-        w = unet(yplane, p, prefix, train, stats)
+        w = unet(yplane, p, prefix, train, stats, norm_groups)
     elif attention:
         w = chan_attention(gazetr_features(yplane, p, prefix), p, prefix + "feed.")
     else:
@@ -403,9 +404,22 @@ def batch_norm_relu(x: torch.Tensor, p: Params, prefix: str, train: bool, stats:
     return torch.relu(x * scale[None, :, None, None] + shift[None, :, None, None])
 
 
-def double_conv(x: torch.Tensor, p: Params, prefix: str, train: bool, stats: Optional[dict] = None) -> torch.Tensor:
-    """prefix ends in 'double_conv.': Sequential indices 0 conv, 1 BN, 3 conv, 4 BN (unet_blocks.py:16-28)."""
+def group_norm_relu(x: torch.Tensor, p: Params, prefix: str, groups: int, eps: float = 1e-5) -> torch.Tensor:
+    """GroupNorm + ReLU (not in the reference): statistics over the pixels and the channels of a group of one image."""
+    B, C, H, W = x.shape
+    v = x.reshape(B, groups, -1)
+    d = v - v.mean(dim=-1, keepdim=True)
+    xh = (d / torch.sqrt((d * d).mean(dim=-1, keepdim=True) + eps)).reshape(x.shape)
+    return torch.relu(xh * p[prefix + "weight"][None, :, None, None] + p[prefix + "bias"][None, :, None, None])
+
+
+def double_conv(x: torch.Tensor, p: Params, prefix: str, train: bool, stats: Optional[dict] = None, groups: int = 0) -> torch.Tensor:
+    """prefix ends in 'double_conv.': Sequential indices 0 conv, 1 BN, 3 conv, 4 BN (unet_blocks.py:16-28).
+    groups > 0: GroupNorm in the place of both BatchNorms."""
     h = F.conv2d(x, p[prefix + "0.weight"], None, padding=1)
+    if groups:
+        h = F.conv2d(group_norm_relu(h, p, prefix + "1.", groups), p[prefix + "3.weight"], None, padding=1)
+        return group_norm_relu(h, p, prefix + "4.", groups)
     h = batch_norm_relu(h, p, prefix + "1.", train, stats)
     h = F.conv2d(h, p[prefix + "3.weight"], None, padding=1)
     return batch_norm_relu(h, p, prefix + "4.", train, stats)
@@ -440,19 +454,20 @@ def anchor_attention(x: torch.Tensor, p: Params, prefix: str, heads: int) -> tor
 UNET_HEADS = {"att1": 2, "att2": 2, "att3": 4, "att4": 4}                    # unet.py:23-26
 
 
-def unet(x: torch.Tensor, p: Params, prefix: str = "", train: bool = False, stats: Optional[dict] = None) -> torch.Tensor:
+def unet(x: torch.Tensor, p: Params, prefix: str = "", train: bool = False, stats: Optional[dict] = None,
+         groups: int = 0) -> torch.Tensor:
     """UNet(in, P).forward (unet.py:30-42): x [B,1,H,W] -> [B,P,H,W]; H, W >= 16 (sizes that are not multiples of 16:
     the pooling floors and the upsampled tensor is zero-padded to the skip's size)."""
-    xs = [double_conv(x, p, prefix + "proj.double_conv.", train, stats)]
+    xs = [double_conv(x, p, prefix + "proj.double_conv.", train, stats, groups)]
     for i in range(1, 5):
-        xs.append(double_conv(F.max_pool2d(xs[-1], 2), p, prefix + f"down{i}.maxpool_conv.1.double_conv.", train, stats))
+        xs.append(double_conv(F.max_pool2d(xs[-1], 2), p, prefix + f"down{i}.maxpool_conv.1.double_conv.", train, stats, groups))
     y = xs[4]
     for i in range(1, 5):
         skip = anchor_attention(xs[4 - i], p, prefix + f"att{5 - i}.", UNET_HEADS[f"att{5 - i}"])
         up = F.conv_transpose2d(y, p[prefix + f"up{i}.up.weight"], p[prefix + f"up{i}.up.bias"], stride=2)
         dy, dx = skip.shape[2] - up.shape[2], skip.shape[3] - up.shape[3]          # unet_blocks.py:68-73
         up = F.pad(up, [dx // 2, dx - dx // 2, dy // 2, dy - dy // 2])
-        y = double_conv(torch.cat([skip, up], dim=1), p, prefix + f"up{i}.conv.double_conv.", train, stats)
+        y = double_conv(torch.cat([skip, up], dim=1), p, prefix + f"up{i}.conv.double_conv.", train, stats, groups)
     return F.conv2d(y, p[prefix + "reproj.conv.weight"], p[prefix + "reproj.conv.bias"])
 
 

@@ -196,6 +196,69 @@ extern "C" int ksr_adam_step_dev(float* params, const float* grads, float* exp_a
     return KSR_OK;
 }
 
+namespace {
+
+constexpr int ADAM_RUNS = 128;
+struct AdamRuns { long first[ADAM_RUNS]; int len[ADAM_RUNS]; };
+
+// Adam over parts of the flat buffers (run blockIdx.y), the arithmetic of adam_kernel / adam_dev_kernel
+__global__ void __launch_bounds__(256) adam_runs_kernel(AdamRuns r, float* __restrict__ p, const float* __restrict__ g,
+                                                        float* __restrict__ m, float* __restrict__ v, float lr,
+                                                        const float* __restrict__ lr_dev, float beta1, float beta2, float eps,
+                                                        float wd, float bc1, float bc2_sqrt,
+                                                        const unsigned long long* __restrict__ step_dev, float gscale) {
+    if (step_dev) {
+        const double st = (double)*step_dev;
+        bc1 = (float)(1.0 - pow((double)beta1, st));
+        bc2_sqrt = (float)sqrt(1.0 - pow((double)beta2, st));
+        lr = *lr_dev;
+    }
+    const long first = r.first[blockIdx.y];
+    for (int k = (int)(blockIdx.x * blockDim.x + threadIdx.x); k < r.len[blockIdx.y]; k += (int)(gridDim.x * blockDim.x)) {
+        const long i = first + k;
+        float gi = g[i] * gscale;
+        const float pi = p[i];
+        if (wd != 0.f) gi += wd * pi;
+        const float mi = beta1 * m[i] + (1.f - beta1) * gi;
+        const float vi = beta2 * v[i] + (1.f - beta2) * gi * gi;
+        m[i] = mi;
+        v[i] = vi;
+        const float denom = sqrtf(vi) / bc2_sqrt + eps;
+        p[i] = pi - (lr / bc1) * (mi / denom);
+    }
+}
+
+}  // namespace
+
+extern "C" int ksr_adam_step_runs(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, const int64_t* runs, int n_runs,
+                                  float lr, const float* lr_dev, float beta1, float beta2, float eps, float weight_decay, int step,
+                                  const uint64_t* step_dev, float grad_scale, hipStream_t stream) {
+    KSR_CHECK_ARG(params && grads && exp_avg && exp_avg_sq && (runs || n_runs == 0) && n_runs >= 0, "adam_step_runs: bad argument");
+    KSR_CHECK_ARG((lr_dev != nullptr) == (step_dev != nullptr) && (step_dev || step >= 1), "adam_step_runs: a step count from 1, or lr_dev and step_dev");
+    for (int i = 0; i < n_runs; ++i)
+        KSR_CHECK_ARG(runs[2 * i] >= 0 && runs[2 * i + 1] >= 0 && runs[2 * i + 1] < (1ll << 31), "adam_step_runs: run %d is (%lld, %lld)", i,
+                      (long long)runs[2 * i], (long long)runs[2 * i + 1]);
+    const float bc1 = (float)(1.0 - pow((double)beta1, (double)step));
+    const float bc2_sqrt = (float)sqrt(1.0 - pow((double)beta2, (double)step));
+    for (int base = 0; base < n_runs; base += ADAM_RUNS) {
+        AdamRuns r{};
+        const int n = n_runs - base < ADAM_RUNS ? n_runs - base : ADAM_RUNS;
+        int64_t longest = 0;
+        for (int i = 0; i < n; ++i) {
+            r.first[i] = (long)runs[2 * (base + i)];
+            r.len[i] = (int)runs[2 * (base + i) + 1];
+            if (r.len[i] > longest) longest = r.len[i];
+        }
+        if (!longest) continue;
+        const int64_t gx = (longest + 255) / 256;
+        hipLaunchKernelGGL(adam_runs_kernel, dim3((unsigned)(gx < 256 ? gx : 256), (unsigned)n), dim3(256), 0, stream, r, params, grads,
+                           exp_avg, exp_avg_sq, lr, lr_dev, beta1, beta2, eps, weight_decay, bc1, bc2_sqrt,
+                           reinterpret_cast<const unsigned long long*>(step_dev), grad_scale);
+        KSR_LAUNCH_CHECK("adam_step_runs");
+    }
+    return KSR_OK;
+}
+
 // ------------------------------------------------------------------------------------------ RCCL
 extern "C" int ksr_comm_unique_id(void* out128) {
     KSR_CHECK_ARG(out128 != nullptr, "comm_unique_id: null pointer");

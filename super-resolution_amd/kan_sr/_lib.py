@@ -37,7 +37,7 @@ class _Proxy:
 
     def __getattr__(self, name):
         fn = getattr(self._cdll, name)
-        if PROFILE is None or not name.endswith(("_fwd", "_bwd", "_up", "_wgrad", "_sum", "colreduce", "_token", "_attn", "_loss", "_step", "outer2", "_batched", "_apply", "_entries", "_ycbcr", "_rgb", "_grad", "_finalize", "_mix", "_merge", "_dgrad", "_batch", "_wg", "_v", "_l1", "_input", "_img", "_kan", "_flush", "_groups", "_lnf", "_bwd_dx")):
+        if PROFILE is None or not name.endswith(("_fwd", "_bwd", "_up", "_wgrad", "_sum", "colreduce", "_token", "_attn", "_loss", "_step", "outer2", "_batched", "_apply", "_entries", "_ycbcr", "_rgb", "_grad", "_finalize", "_mix", "_merge", "_dgrad", "_batch", "_wg", "_v", "_l1", "_input", "_img", "_kan", "_flush", "_groups", "_lnf", "_bwd_dx", "_runs")):
             return fn
 
         def timed(*args):
@@ -100,7 +100,7 @@ EXPORTS = [
     "ksr_batch_attn_bwd", "ksr_tx_bwd_wg_slab_floats", "ksr_batch_tx_layer_bwd_out_wg", "ksr_wgrad_affine_input",
     "ksr_gate_pw_bwd_v", "ksr_fn1_bwd_stem_v", "ksr_dwconv_wgrad_v", "ksr_in_proj_bwd", "ksr_in_proj_bwd_wg", "ksr_in_proj_bwd_wg_slab_floats", "ksr_gate_pw_bwd", "ksr_gate_pw_bwd_wg", "ksr_pw2_bwd_wg", "ksr_pw1_bwd_wg", "ksr_fused_wgrad_slab_floats", "ksr_fn1_bwd", "ksr_pw2_bwd", "ksr_pw1_bwd",
     "ksr_wgrad_slab_floats", "ksr_wgrad", "ksr_colreduce", "ksr_dwconv_wgrad", "ksr_stem_scalar_wgrad", "ksr_outer2",
-    "ksr_l1_y_loss", "ksr_l1_y_loss_static", "ksr_adam_step", "ksr_adam_step_dev", "ksr_set_dropout_seed_source", "ksr_comm_unique_id", "ksr_comm_init", "ksr_allreduce_sum", "ksr_comm_nranks",
+    "ksr_l1_y_loss", "ksr_l1_y_loss_static", "ksr_adam_step", "ksr_adam_step_dev", "ksr_adam_step_runs", "ksr_set_dropout_seed_source", "ksr_comm_unique_id", "ksr_comm_init", "ksr_allreduce_sum", "ksr_comm_nranks",
     "ksr_comm_destroy",
     "ksr_pointwise_bwd", "ksr_chan_dw_fwd", "ksr_chan_dw_bwd", "ksr_chan_dw_bwd_dx", "ksr_gram_slab_floats", "ksr_gram_batched",
     "ksr_chan_soft_fwd", "ksr_chan_soft_bwd", "ksr_sum_entries", "ksr_chan_apply",

@@ -51,6 +51,9 @@ def adam_state_dict(ts: TrainStep) -> dict:
     group = {"lr": ts.lr, "betas": tuple(ts.betas), "eps": ts.eps, "weight_decay": ts.wd, "amsgrad": False,
              "maximize": False, "foreach": None, "capturable": False, "differentiable": False, "fused": None,
              "initial_lr": ts.base_lr, "params": list(range(len(names)))}
+    if ts.optimizer == "muon":
+        # exp_avg of these parameters is Muon's momentum, their exp_avg_sq is zero: not an Adam state to resume with
+        group["muon"] = {"momentum": ts.muon_momentum, "params": [i for i, n in enumerate(names) if n in set(ts.muon_names)]}
     return {"state": state, "param_groups": [group]}
 
 
@@ -58,6 +61,14 @@ def load_adam_state(ts: TrainStep, opt_state: dict) -> None:
     """Inverse of adam_state_dict: copies the moments of the trained layer into the flat buffers."""
     names = [n for n, _ in ts.model.named_parameters()]
     named = dict(ts.model.named_parameters())
+    muon = (opt_state.get("param_groups") or [{}])[0].get("muon")
+    theirs = sorted(muon["params"]) if muon else []
+    ours = sorted(i for i, n in enumerate(names) if ts.optimizer == "muon" and n in set(ts.muon_names))
+    if theirs != ours:
+        raise KsrError(f"the checkpoint's optimizer updates {len(theirs)} matrices by Muon, this TrainStep {len(ours)}"
+                       + ("" if len(theirs) != len(ours) else " (other ones)"))
+    if muon:
+        ts.muon_momentum = float(muon["momentum"])
     off = 0
     steps = 0
     for n in ts.order:

@@ -81,11 +81,11 @@ class GazeTR(_Container):                   # conv_sep_kan/gazetr.py:69-98
 
 
 class ConvSepKanEncoder(_Container):        # conv_sep_kan/conv_sep_kan_encoder.py:12-17
-    def __init__(self, in_channels, out_channels, attention=False, backbone="gazetr"):
+    def __init__(self, in_channels, out_channels, attention=False, backbone="gazetr", norm="batch", norm_groups=2):
         super().__init__()
         if backbone == "unet":              # the backbone conv_sep_kan_encoder.py:7 imports beside GazeTR
             from .unet import UNet
-            self.encoder = UNet(in_channels, out_channels)
+            self.encoder = UNet(in_channels, out_channels, norm=norm, norm_groups=norm_groups)
         else:
             self.encoder = GazeTR(in_channels, out_channels, attention)
 
@@ -100,10 +100,10 @@ class ConvSepKanCell(_Container):           # conv_sep_kan/conv_sep_kan_cells.py
 
 class ConvSepKanLayer(_Container):          # conv_sep_kan/conv_sep_kan_layer.py:7-15
     def __init__(self, in_channels, out_channels, grid_size, spline_order, residual_std, grid_range, attention=False,
-                 backbone="gazetr"):
+                 backbone="gazetr", norm="batch", norm_groups=2):
         super().__init__()
         self.kan_cell = ConvSepKanCell(in_channels, out_channels, grid_size, spline_order, residual_std, grid_range)
-        self.encoder = ConvSepKanEncoder(in_channels, self.kan_cell.size, attention, backbone)
+        self.encoder = ConvSepKanEncoder(in_channels, self.kan_cell.size, attention, backbone, norm, norm_groups)
 
 
 # cfg-4 wiring: evaluate the attention head's per-image 1x1 map inside the fused feed+KAN kernel (False: materialise the
@@ -122,15 +122,21 @@ class ConvSepKan(nn.Module):
 
     backbone="unet" (keyword only) selects the reference's UNet (conv_sep_kan/unet.py) as the hyper-encoder in place
     of GazeTR, i.e. `self.encoder = UNet(in_channels, out_channels)` at conv_sep_kan_encoder.py:17; state_dict keys
-    `layers.N.encoder.encoder.{proj,down1..4,up1..4,att1..4,reproj}.*`.  Forward and backward (fp32 only)."""
+    `layers.N.encoder.encoder.{proj,down1..4,up1..4,att1..4,reproj}.*`.  Forward and backward (fp32 only).
+
+    norm="group" (keyword only, with backbone="unet"; not in the reference): GroupNorm over norm_groups groups of channels in
+    place of the UNet's BatchNorm2d: no statistics across images or ranks, no running statistics, train and eval are equal."""
 
     def __init__(self, in_channels: list, out_channels: list, kernel_sizes: list, grid_size, spline_order,
-                 residual_std, grid_range, upscale, *, attention: bool = False, backbone: str = "gazetr"):
+                 residual_std, grid_range, upscale, *, attention: bool = False, backbone: str = "gazetr",
+                 norm: str = "batch", norm_groups: int = 2):
         super().__init__()
         if backbone not in ("gazetr", "unet"):
             raise KsrError(f"backbone must be 'gazetr' or 'unet', got {backbone!r}")
         if backbone == "unet" and attention:
             raise KsrError("attention=True replaces GazeTR's feed conv: it does not combine with backbone='unet'")
+        if norm != "batch" and backbone != "unet":
+            raise KsrError("norm applies to the UNet's blocks: it needs backbone='unet'")
         self.upscale = upscale
         self.attention = attention
         self.backbone = backbone
@@ -142,7 +148,7 @@ class ConvSepKan(nn.Module):
         self.shuffle = nn.PixelShuffle(upscale)          # kept for module-tree parity; no parameters
         for in_ch, out_ch in zip(in_channels, out_channels):
             self.layers.append(ConvSepKanLayer(in_ch, out_ch, grid_size, spline_order, residual_std, grid_range,
-                                               attention, backbone))
+                                               attention, backbone, norm, norm_groups))
         if len(self.layers) == 0:
             raise KsrError("ConvSepKan needs at least one layer")
         # Every layer is fed the Y plane and only the last layer's output survives the reference's

@@ -25,6 +25,7 @@ from . import _lib
 from ._lib import KsrError, check, lib, ptr, stream
 from .autograd import PARAM_ORDER, backward_all
 from .engine import TX_PARAM_NAMES
+from .muon import as_matrix, muon_update
 
 # gradient-completion order of the parameter groups (see module docstring)
 _TAIL = (["feed.weight", "feed.bias"]
@@ -59,6 +60,25 @@ def shard_batch(global_batch: int, world_size: int, rank: int):
     base, rem = divmod(global_batch, world_size)
     lo = rank * base + min(rank, rem)
     return lo, lo + base + (1 if rank < rem else 0)
+
+
+def takes_muon(name: str, shape: torch.Size) -> bool:
+    """Whether a hyper-encoder parameter is a hidden dense map, for which Muon's update is meant: matrices (convolutions as
+    [out, in * kh * kw]) with both sides of 16 or more - not depthwise filters ([C, 9]), not the one-channel stem - other than
+    the head that produces the KAN parameters (feed, reproj)."""
+    m = as_matrix(shape)
+    return m is not None and min(m) >= 16 and not name.startswith(("feed.", "reproj."))
+
+
+def flat_runs(parts) -> ctypes.Array:
+    """(offset, numel) parts in ascending order -> the fewest (first, length) pairs that cover them, as a C array."""
+    runs: List[int] = []
+    for off, n in parts:
+        if runs and runs[-2] + runs[-1] == off:
+            runs[-1] += n
+        else:
+            runs += [off, n]
+    return (c_int64 * len(runs))(*runs)
 
 
 class RcclComm:
@@ -106,8 +126,14 @@ class TrainStep:
 
     def __init__(self, model, world_size: int = 1, rank: int = 0, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.0, comm=None, loss: str = "l1", capture: bool = False,
-                 device_state: Optional[bool] = None):
-        """capture: after two ordinary steps at a given input shape, forward + loss + backward (and, when nothing has
+                 device_state: Optional[bool] = None, optimizer: str = "adam", muon_momentum: float = 0.95,
+                 muon_params: Optional[Callable[[str, torch.Size], bool]] = None):
+        """optimizer: "adam" for every parameter, or "muon": the weight matrices that muon_params(name, shape) picks (default:
+        takes_muon) are updated along the orthogonalised momentum (kan_sr.muon.muon_update, momentum muon_momentum), all others
+        by Adam.  Both use `lr`; weight_decay is Adam's L2 term for the one and decoupled for the other.  The momenta of the
+        Muon matrices live in their part of exp_avg, so that checkpoints carry them.
+
+        capture: after two ordinary steps at a given input shape, forward + loss + backward (and, when nothing has
         to be exchanged between GPUs first, Adam) are recorded once into a HIP graph and replayed from then on, so
         that the 130 (GazeTR) to 470 (UNet) launches of a step cost the host one call: small per-GPU batches are bound
         by the host's launch rate otherwise.  Up to MAX_GRAPHS input shapes stay recorded.  Inputs are copied into the
@@ -121,7 +147,12 @@ class TrainStep:
         counter.  The UNet encoder (no dropout) keeps Adam outside its graph with by-value arguments."""
         if loss not in ("l1", "l1+ssim"):
             raise KsrError(f"loss must be 'l1' or 'l1+ssim', got {loss!r}")
+        if optimizer not in ("adam", "muon"):
+            raise KsrError(f"optimizer must be 'adam' or 'muon', got {optimizer!r}")
+        if not 0 <= muon_momentum < 1:
+            raise KsrError(f"muon_momentum must be in [0, 1), got {muon_momentum}")
         self.loss_kind = loss
+        self.optimizer, self.muon_momentum = optimizer, muon_momentum
         self.capture = capture
         self._graphs: "OrderedDict" = OrderedDict()
         self.base_lr = lr
@@ -180,6 +211,15 @@ class TrainStep:
                 from .module import FUSED_ATTENTION_HEAD
                 if FUSED_ATTENTION_HEAD:
                     layer.feed.grad_sink = {n[len("feed."):]: self.arena[self.pre + n] for n in self.order if n.startswith("feed.")}
+        if optimizer == "muon":
+            pick = muon_params or takes_muon
+            chosen = [n for n in self.order if as_matrix(named[n].shape) is not None and pick(n, named[n].shape)]
+            if not chosen:
+                raise KsrError("optimizer='muon': no parameter is a matrix that muon_params picks")
+            self._muon = tuple([buf[table[n][0]:table[n][0] + table[n][1]].view(named[n].shape) for n in chosen]
+                               for buf in (self.flat_p, self.flat_g, self.exp_avg))
+            self.muon_names = [self.pre + n for n in chosen]
+            self._adam_runs = flat_runs([table[n] for n in self.order if n not in set(chosen)])
         self._steps = 0
         if self.device_state:
             self._ctr = torch.zeros(1, device=dev, dtype=torch.int64)        # step counter = dropout stream word
@@ -270,6 +310,17 @@ class TrainStep:
 
     def _adam(self) -> None:
         L = lib()
+        if self.optimizer == "muon":
+            runs, dev = self._adam_runs, self.device_state
+            if len(runs):
+                check(L.ksr_adam_step_runs(ptr(self.flat_p), ptr(self.flat_g), ptr(self.exp_avg), ptr(self.exp_avg_sq), runs,
+                                           c_int(len(runs) // 2), c_float(self.lr), ptr(self._lr_dev if dev else None),
+                                           c_float(self.betas[0]), c_float(self.betas[1]), c_float(self.eps), c_float(self.wd),
+                                           c_int(self._steps), c_void_p(self._ctr.data_ptr() if dev else 0),
+                                           c_float(1.0 / self.world_size), stream()), "ksr_adam_step_runs")
+            muon_update(*self._muon, lr=self.lr, momentum=self.muon_momentum, weight_decay=self.wd,
+                        grad_scale=1.0 / self.world_size, lr_dev=self._lr_dev if dev else None)
+            return
         if self.device_state:
             check(L.ksr_adam_step_dev(ptr(self.flat_p), ptr(self.flat_g), ptr(self.exp_avg), ptr(self.exp_avg_sq),
                                       c_int64(self.flat_p.numel()), ptr(self._lr_dev), c_float(self.betas[0]),

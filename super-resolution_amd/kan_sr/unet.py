@@ -18,6 +18,7 @@ import torch
 import torch.nn as nn
 
 from ._lib import KsrError, check, lib, ptr, stream
+from .ops import ACTIVATIONS
 
 
 # One launch for the reductions that finish the plain weight gradients of a backward pass (see UNet._backward)
@@ -30,24 +31,28 @@ def _new(dev, *shape):
 
 
 class DoubleConv(nn.Module):                      # unet_blocks.py:9-28
-    def __init__(self, cin, cout):
+    def __init__(self, cin, cout, groups=0):
         super().__init__()
+
+        def norm():                               # groups > 0: GroupNorm in place of the reference's BatchNorm2d
+            return nn.GroupNorm(groups, cout) if groups else nn.BatchNorm2d(cout)
+
         self.double_conv = nn.Sequential(
-            nn.Conv2d(cin, cout, kernel_size=3, padding=1, bias=False), nn.BatchNorm2d(cout), nn.ReLU(inplace=True),
-            nn.Conv2d(cout, cout, kernel_size=3, padding=1, bias=False), nn.BatchNorm2d(cout), nn.ReLU(inplace=True))
+            nn.Conv2d(cin, cout, kernel_size=3, padding=1, bias=False), norm(), nn.ReLU(inplace=True),
+            nn.Conv2d(cout, cout, kernel_size=3, padding=1, bias=False), norm(), nn.ReLU(inplace=True))
 
 
 class Down(nn.Module):                            # unet_blocks.py:34-40
-    def __init__(self, cin, cout):
+    def __init__(self, cin, cout, groups=0):
         super().__init__()
-        self.maxpool_conv = nn.Sequential(nn.MaxPool2d(2), DoubleConv(cin, cout))
+        self.maxpool_conv = nn.Sequential(nn.MaxPool2d(2), DoubleConv(cin, cout, groups))
 
 
 class Up(nn.Module):                              # unet_blocks.py:46-63 (bilinear=False)
-    def __init__(self, cin, cout):
+    def __init__(self, cin, cout, groups=0):
         super().__init__()
         self.up = nn.ConvTranspose2d(cin, cin // 2, kernel_size=2, stride=2)
-        self.conv = DoubleConv(cin, cout)
+        self.conv = DoubleConv(cin, cout, groups)
 
 
 class OutConv(nn.Module):                         # unet_blocks.py:81-85
@@ -132,13 +137,23 @@ class _GatherPlan:
 
 
 class UNet(nn.Module):
-    """UNet(in_channels, out_channels) as in the reference; in_channels must be 1 and out_channels a multiple of 4."""
+    """UNet(in_channels, out_channels) as in the reference; in_channels must be 1 and out_channels a multiple of 4.
 
-    def __init__(self, in_channels, out_channels):
+    norm="group" (not in the reference): every BatchNorm2d is a GroupNorm of norm_groups (1, 2 or 4) groups, the same state_dict
+    keys without the running statistics.  Its normalised tensors are written out (statistics per image cannot be folded into
+    the next convolution's loads as BatchNorm's per-channel affine form is)."""
+
+    def __init__(self, in_channels, out_channels, norm="batch", norm_groups=2):
         super().__init__()
-        self.proj = DoubleConv(in_channels, 4)
-        self.down1, self.down2, self.down3, self.down4 = Down(4, 8), Down(8, 16), Down(16, 32), Down(32, 64)
-        self.up1, self.up2, self.up3, self.up4 = Up(64, 32), Up(32, 16), Up(16, 8), Up(8, 4)
+        if norm not in ("batch", "group"):
+            raise KsrError(f"norm must be 'batch' or 'group', got {norm!r}")
+        if norm == "group" and norm_groups not in (1, 2, 4):
+            raise KsrError(f"norm_groups must be 1, 2 or 4 (the shallowest blocks have 4 channels), got {norm_groups!r}")
+        self.norm, g = norm, norm_groups if norm == "group" else 0
+        self.proj = DoubleConv(in_channels, 4, g)
+        self.down1, self.down2, self.down3, self.down4 = Down(4, 8, g), Down(8, 16, g), Down(16, 32, g), Down(32, 64, g)
+        self.up1, self.up2, self.up3, self.up4 = Up(64, 32, g), Up(32, 16, g), Up(16, 8, g), Up(8, 4, g)
+        self._unit: dict = {}          # channels -> (ones, zeros): the affine form of a tensor that is normalised already
         self.att1, self.att2 = SelfAttention(dim=4, num_heads=2), SelfAttention(dim=8, num_heads=2)
         self.att3, self.att4 = SelfAttention(dim=16, num_heads=4), SelfAttention(dim=32, num_heads=4)
         self.reproj = OutConv(4, out_channels)
@@ -159,7 +174,7 @@ class UNet(nn.Module):
         # .to() / .cuda() / .float() replace the buffer tensors: forget everything that was listed or derived from them
         self._counters, self._named = None, None
         self._W, self._prep_ver, self._ptrs, self._sink_key = {}, None, None, None
-        self._bn_eval.clear()
+        self._bn_eval.clear(), self._unit.clear()
         self._prep_plans.clear(), self._emit_plans.clear()
         return super()._apply(fn, *args, **kwargs)
 
@@ -418,8 +433,53 @@ class UNet(nn.Module):
                                      c_int64(npix), c_int(C), stream()), "ksr_unet_bn_relu_bwd")
         return dx
 
+    def _gn(self, gn: nn.GroupNorm, raw, B, S):
+        """relu(GroupNorm(raw)) of raw [B, H, W, C] -> (output, per-image statistics for the backward)."""
+        L = lib()
+        C, G = gn.num_channels, gn.num_groups
+        out, stats = torch.empty_like(raw), _new(raw.device, B, G, 2)
+        ws = _new(raw.device, int(L.ksr_group_norm_ws_floats(c_int64(B), c_int64(S), c_int(C), c_int(G), c_int(0))))
+        check(L.ksr_group_norm_fwd(ptr(raw), c_int64(S * C), c_int64(C), ptr(gn.weight.detach()), ptr(gn.bias.detach()), ptr(out),
+                                   ptr(stats), ptr(ws), c_int64(B), c_int64(S), c_int(C), c_int(G), c_float(gn.eps),
+                                   c_int(ACTIVATIONS["relu"]), c_int(0), stream()), "ksr_group_norm_fwd")
+        return out, stats
+
+    def _gn_bwd(self, gn: nn.GroupNorm, dout, raw, stats, B, S, names):
+        """-> gradient of raw; the affine parameters' gradients go to names = (weight name, bias name)."""
+        L = lib()
+        C, G = gn.num_channels, gn.num_groups
+        dx = torch.empty_like(raw)
+        ws = _new(raw.device, int(L.ksr_group_norm_ws_floats(c_int64(B), c_int64(S), c_int(C), c_int(G), c_int(1))))
+        check(L.ksr_group_norm_bwd(ptr(raw), c_int64(S * C), c_int64(C), ptr(dout), c_int64(S * C), c_int64(C),
+                                   ptr(gn.weight.detach()), ptr(gn.bias.detach()), ptr(stats), ptr(dx), ptr(self._gdst[names[0]]),
+                                   ptr(self._gdst[names[1]]), ptr(ws), c_int64(B), c_int64(S), c_int(C), c_int(G),
+                                   c_int(ACTIVATIONS["relu"]), c_int(0), stream()), "ksr_group_norm_bwd")
+        return dx
+
+    def _double_conv_gn(self, key, seq, src0, c0, B, H, W, src1, c1, pool, tape):
+        cout = seq[0].out_channels
+        raw1, _ = self._conv(src0, c0, self._W[key + ".0"], cout, B, H, W, src1=src1, c1=c1)
+        mid, st1 = self._gn(seq[1], raw1, B, H * W)
+        raw2, _ = self._conv(mid, cout, self._W[key + ".3"], cout, B, H, W)
+        out, st2 = self._gn(seq[4], raw2, B, H * W)
+        pooled = None
+        if pool:
+            # the pooling of the BatchNorm path's kernel; scale 1 and shift 0 leave the non-negative values as they are
+            if cout not in self._unit:
+                self._unit[cout] = (torch.ones(cout, device=out.device), torch.zeros(cout, device=out.device))
+            one, zero = self._unit[cout]
+            pooled = _new(src0.device, B, H // 2, W // 2, cout)
+            check(lib().ksr_unet_bn_relu_fwd(ptr(out), ptr(one), ptr(zero), ptr(out), ptr(pooled), c_int(B), c_int(H), c_int(W),
+                                             c_int(cout), stream()), "ksr_unet_bn_relu_fwd")
+        if tape is not None:
+            tape[key] = dict(src0=src0, c0=c0, src1=src1, c1=c1, raw1=raw1, aff1=st1, mid=mid, raw2=raw2, aff2=st2, out=out,
+                             dims=(B, H, W), cout=cout, train=True)
+        return out, pooled
+
     def _double_conv(self, key, dc: DoubleConv, src0, c0, B, H, W, train, src1=None, c1=0, pool=False, tape=None):
         seq = dc.double_conv
+        if self.norm == "group":
+            return self._double_conv_gn(key, seq, src0, c0, B, H, W, src1, c1, pool, tape)
         cout = seq[0].out_channels
         w1, w2 = self._W[key + ".0"], self._W[key + ".3"]
         raw1, part1 = self._conv(src0, c0, w1, cout, B, H, W, src1=src1, c1=c1, stats=train)
@@ -444,10 +504,18 @@ class UNet(nn.Module):
         c, c0, c1, train = t["cout"], t["c0"], t["c1"], t["train"]
         npix = B * H * W
         n1, n2 = (key + ".double_conv.1.weight", key + ".double_conv.1.bias"), (key + ".double_conv.4.weight", key + ".double_conv.4.bias")
-        draw2 = self._bn_bwd(seq[4], dout, t["raw2"], t["aff2"], train, npix, n2)
-        self._wgrad(draw2, c, B, H, W, a0=t["raw1"], ca0=c, affine=t["aff1"][:2], Ha=H, Wa=W, out=self._KG[key + ".3"])
+        group = self.norm == "group"
+        if group:
+            draw2 = self._gn_bwd(seq[4], dout, t["raw2"], t["aff2"], B, H * W, n2)
+            self._wgrad(draw2, c, B, H, W, a0=t["mid"], ca0=c, Ha=H, Wa=W, out=self._KG[key + ".3"])
+        else:
+            draw2 = self._bn_bwd(seq[4], dout, t["raw2"], t["aff2"], train, npix, n2)
+            self._wgrad(draw2, c, B, H, W, a0=t["raw1"], ca0=c, affine=t["aff1"][:2], Ha=H, Wa=W, out=self._KG[key + ".3"])
         dmid, _ = self._conv(draw2, c, self._W[key + ".3.T"], c, B, H, W)
-        draw1 = self._bn_bwd(seq[1], dmid, t["raw1"], t["aff1"], train, npix, n1)
+        if group:
+            draw1 = self._gn_bwd(seq[1], dmid, t["raw1"], t["aff1"], B, H * W, n1)
+        else:
+            draw1 = self._bn_bwd(seq[1], dmid, t["raw1"], t["aff1"], train, npix, n1)
         self._wgrad(draw1, c, B, H, W, a0=t["src0"], ca0=c0, a1=t["src1"], ca1=c1, Ha=H, Wa=W, out=self._KG[key + ".0"])
         if not need_input_grad:
             return None, None
@@ -568,7 +636,8 @@ class UNet(nn.Module):
         if train:
             if self._counters is None:
                 self._counters = [m.num_batches_tracked for m in self.modules() if isinstance(m, nn.BatchNorm2d)]
-            torch._foreach_add_(self._counters, 1)
+            if self._counters:
+                torch._foreach_add_(self._counters, 1)
         return out.view(B * H * W, -1)
 
     def _backward(self, tape, dw, want_input_grad=False):

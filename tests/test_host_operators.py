@@ -99,3 +99,33 @@ def test_muon_refuses_at_the_abi():
     assert need > 0 and L.ksr_muon_ws_bytes(one(rows=64, cols=1024), c_int(1), c_int(1)) == 0
     assert call(one(rows=100, cols=100), ws=c_void_p(A + 8), ws_bytes=need) == -1
     assert call(one(rows=0)) == 0 and call(None, count=0) == 0
+
+
+def test_flat_runs_and_the_matrices_that_muon_takes():
+    from kan_sr.train import flat_runs, takes_muon
+    assert list(flat_runs([(0, 4), (4, 6), (12, 1), (13, 2)])) == [0, 10, 12, 3] and len(flat_runs([])) == 0
+    pick = [("ffn3.pointwise1.weight", (64, 64, 1, 1), True), ("ffn3.depthwise.weight", (64, 1, 3, 3), False), ("feed.weight", (160, 64, 1, 1), False),
+            ("encoder.layers.0.linear1.weight", (32, 64), True), ("encoder.norm.weight", (64,), False), ("ffn1.pointwise2.weight", (64, 1, 1, 1), False),
+            ("reproj.conv.weight", (160, 4, 1, 1), False), ("down4.maxpool_conv.1.double_conv.0.weight", (64, 32, 3, 3), True)]
+    assert all(takes_muon(n, torch.Size(s)) == want for n, s, want in pick)
+
+
+def test_adam_runs_refusals():
+    from kan_sr import _lib
+    L, fake = _lib.lib(), c_void_p(1 << 20)
+
+    def call(runs, n, step=1, lr_dev=None, step_dev=None):
+        return L.ksr_adam_step_runs(fake, fake, fake, fake, runs, c_int(n), c_float(1.0), lr_dev, c_float(0.9), c_float(0.9), c_float(1e-8),
+                                    c_float(0.0), c_int(step), step_dev, c_float(1.0), None)
+
+    two = (c_int64 * 2)(0, 4)
+    assert call(None, 1) == -1 and call(two, -1) == -1 and call(two, 1, step=0) == -1 and call(two, 1, lr_dev=fake) == -1
+    assert call((c_int64 * 2)(-1, 4), 1) == -1 and call((c_int64 * 2)(0, 1 << 31), 1) == -1
+    assert call(two, 0) == 0 and call((c_int64 * 2)(0, 0), 1) == 0
+
+
+def test_group_norm_unet_has_the_batch_norm_keys_without_running_statistics():
+    from kan_sr.unet import UNet
+    batch, group = UNet(1, 40).state_dict(), UNet(1, 40, norm="group").state_dict()
+    assert set(group) == {k for k in batch if "running" not in k and "num_batches" not in k}
+    assert all(group[k].shape == batch[k].shape for k in group)
