@@ -25,7 +25,6 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float S = 1024.f, INV_S = 1.f / 1024.f;     // values up to 30 (checked on the host) fit f16
 constexpr int MAX_STEPS = 32, MAX_MATS = 40;
-constexpr int NORM_PARTS = 64;                        // partial sums of squares per matrix (large path)
 
 struct Mat {
     const void* src;          // U, or the gradient
@@ -348,73 +347,162 @@ __global__ void __launch_bounds__(512) ns_small_kernel(Mats p) {
 }
 
 // ================================================================================================ large matrices
+// All matrices of a call that are not small run together, whatever their shapes: per step one launch for A, one for B and one for
+// the next X, over the tiles of all of them.
 // Buffers of one matrix, padded to the tile in both directions with zeros that every step reproduces (A, B and X of a zero row
 // or column are zero), so that no product needs a bounds check:  X [mp][np] and X^T [np][mp] (twice), R and B [mp][mp].  With X
 // in both orders each of the three products contracts the contiguous dimension of both operands.
+constexpr int MAX_LARGE = 24;
+constexpr int NORM_PARTS = 256;                         // partial sums of squares per matrix, at most
+constexpr int CUS = 256, SLOTS = 1024;                  // SLOTS: partial tiles of the products that are cut along k, at most
+
+struct LMat {
+    long off;                       // of the first matrix's buffers in the workspace
+    int m, n, mp, np, tall;
+    int sub0, nsub;                 // matrices sub0 .. sub0 + nsub - 1 of the entry's batch
+    int parts;
+    int first, sym, full;           // matrices, tiles of the lower triangles, tiles of X in the entries before this one
+};
 struct Large {
     char* ws;
-    long per;                       // bytes per matrix
-    long o_x, o_xt[2], o_r, o_b, o_d, o_e, o_xi, o_sq;
-    int m, n, mp, np, tall, tile, batch, base;   // base: index of the first matrix of this launch among p.m
+    long o_part;                    // fp32 partial tiles, then SLOTS counters
+    int count, tile, split;
+    LMat e[MAX_LARGE];
 };
 
-struct NormArgs { Mats p; Large l; };
+__host__ __device__ inline long align256(long v) { return (v + 255) / 256 * 256; }
+struct Offsets {
+    long x, xt0, xt1, r, b, d, e, xi, sq, per;
+    __host__ __device__ Offsets(int mp, int np, bool split) {
+        const long xp = 2l * mp * np, ap = 2l * mp * mp;
+        long o = 0;
+        x = o; o += align256(xp * (split ? 2 : 1));
+        xt0 = o; o += align256(2 * xp);
+        xt1 = o; o += align256(2 * xp);
+        r = o; o += align256(ap * (split ? 2 : 1));
+        b = o; o += align256(ap * (split ? 2 : 1));
+        d = o; o += align256(4l * mp);
+        e = o; o += align256(4l * mp);
+        xi = o; o += align256(4l * (MAX_STEPS + 1));
+        sq = o; o += align256(8l * NORM_PARTS);
+        per = o;
+    }
+    __device__ __forceinline__ long xt(int k) const { return (k & 1) ? xt1 : xt0; }       // X^T before step k
+};
 
-// partial sums of squares (64-bit), the momentum update on the way
+struct LargeArgs { Step s; Large l; Mat m[MAX_LARGE]; int k, whole, cut; };
+
+// partial sums of squares (64-bit), the momentum update on the way; grid (NORM_PARTS, matrices)
 template <int MODE>
-__global__ void __launch_bounds__(256) ns_norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(256) ns_norm_kernel(LargeArgs a) {
     __shared__ double sq[4];
-    int sub;
-    const Mat& mt = find(a.p, a.l.base + (int)blockIdx.y, sub);
-    // threads walk the contiguous dimension of U
+    int q = 0;
+    while (q + 1 < a.l.count && (int)blockIdx.y >= a.l.e[q + 1].first) ++q;
+    const LMat& le = a.l.e[q];
+    const Mat& mt = a.m[q];
+    if ((int)blockIdx.x >= le.parts) return;
+    const int at = (int)blockIdx.y - le.first, sub = le.sub0 + at;
+    // threads walk the contiguous dimension of U, TX of them along it and 256 / TX along the other
     const bool by_col = mt.cs <= mt.rs;
     const int inner = by_col ? mt.cols : mt.rows, outer = by_col ? mt.rows : mt.cols;
+    const long os = by_col ? mt.rs : mt.cs, is = by_col ? mt.cs : mt.rs, base = (long)sub * mt.bs;
+    // four at a time where the addresses allow it
+    const uintptr_t bytes = MODE == BF16 ? 8 : 16;
+    const bool vec = is == 1 && inner % 4 == 0 && os % 4 == 0 && base % 4 == 0 && (uintptr_t)mt.src % bytes == 0 &&
+                     (MODE != MUON || (by_col && (uintptr_t)mt.mom % 16 == 0));
+    const int cols = vec ? inner / 4 : inner;
+    int tx = 1;
+    while (tx < 256 && tx < cols) tx *= 2;
+    const int ty = 256 / tx, x0 = (int)threadIdx.x % tx, y0 = (int)threadIdx.x / tx;
     double s = 0;
-    for (int o = blockIdx.x; o < outer; o += NORM_PARTS)
-        for (int i = threadIdx.x; i < inner; i += 256) {
-            const double u = load_u<MODE, true>(a.p.s, mt, sub, by_col ? o : i, by_col ? i : o);
-            s = fma(u, u, s);
+    for (int o = (int)blockIdx.x * ty + y0; o < outer; o += le.parts * ty) {
+        if (vec) {
+#pragma unroll 4
+            for (int i = x0; i < cols; i += tx) {
+                float u[4];
+                const long at4 = base + (long)o * os + 4l * i;
+                if constexpr (MODE == BF16) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const __bf16*>(mt.src) + at4);
+                    u[0] = __uint_as_float(w.x << 16); u[1] = __uint_as_float(w.x & 0xffff0000u);
+                    u[2] = __uint_as_float(w.y << 16); u[3] = __uint_as_float(w.y & 0xffff0000u);
+                } else {
+                    const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(mt.src) + at4);
+                    u[0] = w.x; u[1] = w.y; u[2] = w.z; u[3] = w.w;
+                }
+                if constexpr (MODE == MUON) {
+                    float4* mp = reinterpret_cast<float4*>(mt.mom + ((long)sub * mt.rows + o) * mt.cols + 4l * i);
+                    float4 w = *mp;
+                    float* mo = &w.x;
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const float gs = u[z] * a.s.grad_scale;
+                        mo[z] = fmaf(a.s.momentum, mo[z], gs);
+                        u[z] = a.s.nesterov ? fmaf(a.s.momentum, mo[z], gs) : mo[z];
+                    }
+                    *mp = w;
+                }
+#pragma unroll
+                for (int z = 0; z < 4; ++z) s = fma((double)u[z], (double)u[z], s);
+            }
+        } else {
+            for (int i = x0; i < cols; i += tx) {
+                const double u = load_u<MODE, true>(a.s, mt, sub, by_col ? o : i, by_col ? i : o);
+                s = fma(u, u, s);
+            }
         }
+    }
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) sq[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0)
-        reinterpret_cast<double*>(a.l.ws + (long)blockIdx.y * a.l.per + a.l.o_sq)[blockIdx.x] = sq[0] + sq[1] + sq[2] + sq[3];
+    if (threadIdx.x == 0) {
+        const Offsets of(le.mp, le.np, a.l.split != 0);
+        reinterpret_cast<double*>(a.l.ws + le.off + at * of.per + of.sq)[blockIdx.x] = sq[0] + sq[1] + sq[2] + sq[3];
+    }
 }
 
-// X0 in both orders, a 64 x 64 tile per workgroup
+// X0 in both orders, a 64 x 64 tile per workgroup; the counters of the split products are cleared here
 template <int MODE, bool SPLIT>
-__global__ void __launch_bounds__(256) ns_prepare_kernel(NormArgs a) {
+__global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
     __shared__ _Float16 tile[2][64][72];
-    int sub;
-    const Mat& mt = find(a.p, a.l.base + (int)blockIdx.z, sub);
-    char* ws = a.l.ws + (long)blockIdx.z * a.l.per;
-    const double* part = reinterpret_cast<const double*>(ws + a.l.o_sq);
+    __shared__ double part[NORM_PARTS];
+    int q = 0;
+    while (q + 1 < a.l.count && (int)blockIdx.y >= a.l.e[q + 1].first) ++q;
+    const LMat& le = a.l.e[q];
+    const Mat& mt = a.m[q];
+    const int at = (int)blockIdx.y - le.first, sub = le.sub0 + at;
+    const int nj = le.np / 64, ni = le.mp / 64;
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int t = threadIdx.x; t < SLOTS; t += 256) reinterpret_cast<int*>(a.l.ws + a.l.o_part)[t] = 0;
+    if ((int)blockIdx.x >= ni * nj) return;
+    const Offsets of(le.mp, le.np, SPLIT);
+    char* ws = a.l.ws + le.off + at * of.per;
+    if ((int)threadIdx.x < le.parts) part[threadIdx.x] = reinterpret_cast<const double*>(ws + of.sq)[threadIdx.x];
+    __syncthreads();
     double total = 0;
-    for (int i = 0; i < NORM_PARTS; ++i) total += part[i];
+    for (int i = 0; i < le.parts; ++i) total += part[i];
     int e;
-    const float xi0 = scales(a.p.s, total, e);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x <= a.p.s.steps)
-        reinterpret_cast<float*>(ws + a.l.o_xi)[threadIdx.x] = threadIdx.x == 0 ? xi0 : scale_of(a.p.s, total, threadIdx.x);
-    const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
-    const bool across = (mt.cs <= mt.rs) != (a.l.tall != 0);             // whether columns of X are contiguous in U
+    const float xi0 = scales(a.s, total, e);
+    if (blockIdx.x == 0 && (int)threadIdx.x <= a.s.steps)
+        reinterpret_cast<float*>(ws + of.xi)[threadIdx.x] = threadIdx.x == 0 ? xi0 : scale_of(a.s, total, threadIdx.x);
+    const int i0 = (int)blockIdx.x / nj * 64, j0 = (int)blockIdx.x % nj * 64;
+    const bool across = (mt.cs <= mt.rs) != (le.tall != 0);             // whether columns of X are contiguous in U
     for (int t = threadIdx.x; t < 4096; t += 256) {
         const int i = across ? t >> 6 : t & 63, j = across ? t & 63 : t >> 6, gi = i0 + i, gj = j0 + j;
         float v = 0.f;
-        if (gi < a.l.m && gj < a.l.n) v = scaled(load_u<MODE, false>(a.p.s, mt, sub, a.l.tall ? gj : gi, a.l.tall ? gi : gj), e);
+        if (gi < le.m && gj < le.n) v = scaled(load_u<MODE, false>(a.s, mt, sub, le.tall ? gj : gi, le.tall ? gi : gj), e);
         const _Float16 hi = (_Float16)v;
         tile[0][i][j] = hi;
         tile[1][i][j] = (_Float16)(v - (float)hi);
     }
     __syncthreads();
-    const long plane = (long)a.l.mp * a.l.np;
-    _Float16* xt = reinterpret_cast<_Float16*>(ws + a.l.o_xt[0]);
-    _Float16* x = reinterpret_cast<_Float16*>(ws + a.l.o_x);
+    const long plane = (long)le.mp * le.np;
+    _Float16* xt = reinterpret_cast<_Float16*>(ws + of.xt0);
+    _Float16* x = reinterpret_cast<_Float16*>(ws + of.x);
 #pragma unroll
     for (int pl = 0; pl < 2; ++pl)
         for (int t = threadIdx.x; t < 4096; t += 256) {
-            if (SPLIT || pl == 0) x[pl * plane + (long)(i0 + (t >> 6)) * a.l.np + j0 + (t & 63)] = tile[pl][t >> 6][t & 63];
-            xt[pl * plane + (long)(j0 + (t >> 6)) * a.l.mp + i0 + (t & 63)] = tile[pl][t & 63][t >> 6];
+            if (SPLIT || pl == 0) x[pl * plane + (long)(i0 + (t >> 6)) * le.np + j0 + (t & 63)] = tile[pl][t >> 6][t & 63];
+            xt[pl * plane + (long)(j0 + (t >> 6)) * le.mp + i0 + (t & 63)] = tile[pl][t & 63][t >> 6];
         }
 }
 
@@ -423,45 +511,81 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(NormArgs a) {
 //   B_OF_A      P = Q = R, tiles of the lower triangle:   B - diag B, e = a + diag B
 //   X_NEXT      P = B, Q = X^T:                            X, X^T
 //   X_LAST      the same, result or weight update; TALL: P = X^T, Q = B, so that lanes run along U's rows either way
-// Four waves, each (TILE / 2)^2 of the TILE^2 outputs; two stages of BK columns of P and Q in LDS, filled by LDS-DMA one stage
-// ahead.  Rows of a stage hold 16-byte chunks in an order that depends on the row (chunk c of row r at c ^ f(r)), so that the
+// Four waves, each (TILE / 2)^2 of the TILE^2 outputs; NST stages of BK columns of P and Q in LDS, filled by LDS-DMA ahead of
+// their use.  Rows of a stage hold 16-byte chunks in an order that depends on the row (chunk c of row r at c ^ f(r)), so that the
 // eight lanes that read at once hit all banks.
+// Sums: along k in chunks of `chunk_of` columns; a chunk's sum is added to the tile's in the order of k.  Shorter chains of
+// roundings, and the result does not depend on who computes which chunk:
+// Work split: of T tiles the first `whole` = 256 floor(T / 256) have a workgroup each; each chunk of the others has one of its
+// own (`cut`), so that a round that is not full still occupies the chip (528 tiles would otherwise take as long as 768).  Such a
+// workgroup leaves its fp32 sums in the workspace; the one that arrives last adds them in order and goes on with the tile.
 enum { A_OF_X, B_OF_A, X_NEXT, X_LAST };
 
-struct GemmArgs { Mats p; Large l; int k; };
+// 512 columns, more where there would be over 64 chunks; of the unpadded length, so that the tile makes no difference
+__host__ __device__ inline int chunk_of(int k) {
+    int c = 512;
+    while (k > 64 * c) c *= 2;
+    return c;
+}
 
 template <int TILE, bool SPLIT, int KIND>
-__global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
-    constexpr int BK = SPLIT ? 32 : 64, NP = SPLIT ? 2 : 1, W = TILE / 2, NT = W / 32, CH = BK / 8;
+__global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
+    constexpr int BK = SPLIT ? 32 : 64, NP = SPLIT ? 2 : 1, W = TILE / 2, NT = W / 32, CH = BK / 8, NST = TILE == 64 ? 4 : 2;
     constexpr int OPBYTES = TILE * BK * 2, STAGE = 2 * NP * OPBYTES;
     constexpr int STG = TILE + 8;                                       // halves per row of the output tile in LDS
-    constexpr int LDS_BYTES = 2 * STAGE > TILE * STG * 2 ? 2 * STAGE : TILE * STG * 2;
-    __shared__ __attribute__((aligned(16))) char lds[LDS_BYTES];
+    static_assert(NST * STAGE >= TILE * STG * 2, "the output tile reuses the stages");
+    __shared__ __attribute__((aligned(16))) char lds[NST * STAGE];
+    __shared__ int arrived;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1;
-    char* ws = a.l.ws + (long)blockIdx.y * a.l.per;
-    const Large& l = a.l;
+    constexpr bool SYM = KIND == A_OF_X || KIND == B_OF_A;
+    int t, slice = 0, slices = 1, slot = 0, q = 0;      // slot: of the tile's first partial sums
+    if ((int)blockIdx.x < a.whole) {
+        t = (int)ksr_xcd_contiguous(blockIdx.x, (unsigned)a.whole);
+        while (q + 1 < a.l.count && t >= (SYM ? a.l.e[q + 1].sym : a.l.e[q + 1].full)) ++q;
+    } else {
+        // entries whose tiles are cut: each with its own number of chunks
+        int rest = (int)blockIdx.x - a.whole;
+        for (;; ++q) {
+            const LMat& e = a.l.e[q];
+            const int first = SYM ? e.sym : e.full, mt = e.mp / TILE, tiles = e.nsub * (SYM ? mt * (mt + 1) / 2 : mt * (e.np / TILE));
+            const int from = a.whole > first ? a.whole : first, cut = first + tiles - from;       // tiles of this entry in the rest
+            if (cut <= 0) continue;
+            const int ch = chunk_of(KIND == A_OF_X ? e.n : e.m), kp = KIND == A_OF_X ? e.np : e.mp, n = a.cut ? (kp + ch - 1) / ch : 1;
+            if (rest < cut * n || q + 1 == a.l.count) {
+                slices = n;
+                slice = rest % n;
+                slot = (int)blockIdx.x - a.whole - slice;
+                t = from + rest / n;
+                break;
+            }
+            rest -= cut * n;
+        }
+    }
+    const LMat& l = a.l.e[q];
+    t -= SYM ? l.sym : l.full;
+    const int mt = l.mp / TILE, nt = l.np / TILE, per = SYM ? mt * (mt + 1) / 2 : mt * nt;
+    const int at = t / per, sub = l.sub0 + at;
+    t -= at * per;
+    const Offsets of(l.mp, l.np, SPLIT);
+    char* ws = a.l.ws + l.off + at * of.per;
     const bool swap = KIND == X_LAST && l.tall;
-    const int mt = l.mp / TILE;
     int ti, tj;
-    if constexpr (KIND == A_OF_X || KIND == B_OF_A) {
-        const int t = (int)ksr_xcd_contiguous(blockIdx.x, gridDim.x);
+    if constexpr (SYM) {
         ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
         while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
         while (ti * (ti + 1) / 2 > t) --ti;
         tj = t - ti * (ti + 1) / 2;
-    } else {
-        const int t = (int)ksr_xcd_contiguous(blockIdx.x, gridDim.x);
-        if (swap) { ti = t / mt; tj = t % mt; } else { ti = t % mt; tj = t / mt; }
-    }
-    const _Float16* R = reinterpret_cast<const _Float16*>(ws + l.o_r);
-    const _Float16* xt = reinterpret_cast<const _Float16*>(ws + l.o_xt[a.k & 1]);
+    } else if (swap) { ti = t / mt; tj = t % mt; }
+    else { ti = t % mt; tj = t / mt; }
+    const _Float16* R = reinterpret_cast<const _Float16*>(ws + of.r);
+    const _Float16* xt = reinterpret_cast<const _Float16*>(ws + of.xt(a.k));
     const _Float16 *P, *Q;
     long pp, qp;                                        // distance of the lo plane
     int K;
-    if constexpr (KIND == A_OF_X) { P = Q = reinterpret_cast<const _Float16*>(ws + l.o_x); K = l.np; pp = qp = (long)l.mp * l.np; }
+    if constexpr (KIND == A_OF_X) { P = Q = reinterpret_cast<const _Float16*>(ws + of.x); K = l.np; pp = qp = (long)l.mp * l.np; }
     else if constexpr (KIND == B_OF_A) { P = Q = R; K = l.mp; pp = qp = (long)l.mp * l.mp; }
     else {
-        const _Float16* B = reinterpret_cast<const _Float16*>(ws + l.o_b);
+        const _Float16* B = reinterpret_cast<const _Float16*>(ws + of.b);
         P = swap ? xt : B; Q = swap ? B : xt; K = l.mp;
         pp = swap ? (long)l.np * l.mp : (long)l.mp * l.mp;
         qp = swap ? (long)l.mp * l.mp : (long)l.np * l.mp;
@@ -470,18 +594,20 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
     Q += (long)tj * TILE * K;
     // LDS-DMA: one instruction of a wave brings 64 chunks of 16 bytes; lane -> (row, slot), the chunk that belongs there
     constexpr int ROWS = 64 / CH, NI = TILE / ROWS / 4;                 // rows per instruction, instructions per wave and operand plane
+    constexpr int PER_STAGE = 2 * NP * NI;                              // a wave's instructions per stage
     const int drow = lane / CH, dslot = lane % CH;
     auto f = [](int row) { return CH == 8 ? (row & 7) : ((row >> 1) & 3); };
-    auto fill = [&](int st, int kt) {
+    auto fill = [&](int kt) {
+        const int st = kt % NST;
 #pragma unroll
         for (int op = 0; op < 2; ++op)
 #pragma unroll
             for (int pl = 0; pl < NP; ++pl)
 #pragma unroll
-                for (int q = 0; q < NI; ++q) {
-                    const int row = (wave * NI + q) * ROWS + drow;
+                for (int i = 0; i < NI; ++i) {
+                    const int row = (wave * NI + i) * ROWS + drow;
                     const _Float16* src = (op ? Q + pl * qp : P + pl * pp) + (long)row * K + kt * BK + 8 * (dslot ^ f(row));
-                    ksr_dma16<false>(src, lds + st * STAGE + (op * NP + pl) * OPBYTES + (wave * NI + q) * 1024);
+                    ksr_dma16<false>(src, lds + st * STAGE + (op * NP + pl) * OPBYTES + (wave * NI + i) * 1024);
                 }
     };
     auto frag = [&](int st, int op, int pl, int row, int ks) {
@@ -489,23 +615,37 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
         return *reinterpret_cast<const h8*>(lds + st * STAGE + (op * NP + pl) * OPBYTES + row * (BK * 2) + 16 * chunk);
     };
     // hi lo + lo hi have accumulators of their own: added to the large sum one by one they would round it three times a step
-    f32x16 acc[NT][NT] = {}, low[SPLIT ? NT : 1][SPLIT ? NT : 1] = {};
-    const int nk = K / BK;
-    fill(0, 0);
-    for (int kt = 0; kt < nk; ++kt) {
-        ksr_dma_barrier();                              // this stage has landed, the other one has been read by every wave
-        if (kt + 1 < nk) fill((kt + 1) & 1, kt + 1);
-        const int st = kt & 1;
+    f32x16 acc[NT][NT] = {}, low[SPLIT ? NT : 1][SPLIT ? NT : 1] = {}, sum[NT][NT] = {};
+    const int chunk = chunk_of(KIND == A_OF_X ? l.n : l.m) / BK, nk = K / BK;
+    const int k0 = slices > 1 ? slice * chunk : 0, k1 = slices > 1 && k0 + chunk < nk ? k0 + chunk : nk;
+    auto flush = [&]() {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int y = 0; y < NT; ++y) {
+                if constexpr (SPLIT) { acc[x][y] += low[x][y]; low[x][y] = f32x16{}; }
+                sum[x][y] += acc[x][y];
+                acc[x][y] = f32x16{};
+            }
+    };
+    for (int kt = k0; kt < k0 + NST - 1 && kt < k1; ++kt) fill(kt);
+    for (int kt = k0; kt < k1; ++kt) {
+        // stage kt has landed (of the NST - 2 younger ones this wave's transfers may be in flight, if there are that many), and the
+        // stage that is filled next has been read by every wave
+        if (kt + NST - 2 < k1) ksr_dma_barrier_but<PER_STAGE*(NST - 2)>();
+        else ksr_dma_barrier();
+        if (kt + NST - 1 < k1) fill(kt + NST - 1);
+        const int st = kt % NST;
 #pragma unroll
         for (int ks = 0; ks < BK / 16; ++ks) {
             h8 ph[NT], qh[NT], pl[NT], ql[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                ph[t] = frag(st, 0, 0, wr * W + 32 * t + (lane & 31), ks);
-                qh[t] = frag(st, 1, 0, wc * W + 32 * t + (lane & 31), ks);
+            for (int x = 0; x < NT; ++x) {
+                ph[x] = frag(st, 0, 0, wr * W + 32 * x + (lane & 31), ks);
+                qh[x] = frag(st, 1, 0, wc * W + 32 * x + (lane & 31), ks);
                 if constexpr (SPLIT) {
-                    pl[t] = frag(st, 0, 1, wr * W + 32 * t + (lane & 31), ks);
-                    ql[t] = frag(st, 1, 1, wc * W + 32 * t + (lane & 31), ks);
+                    pl[x] = frag(st, 0, 1, wr * W + 32 * x + (lane & 31), ks);
+                    ql[x] = frag(st, 1, 1, wc * W + 32 * x + (lane & 31), ks);
                 }
             }
 #pragma unroll
@@ -519,21 +659,48 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
                     }
                 }
         }
+        if (((kt + 1) & (chunk - 1)) == 0 || kt + 1 == k1) flush();      // chunk is a power of two
     }
-    if constexpr (SPLIT)
+    if (slices > 1) {
+        int* counter = reinterpret_cast<int*>(a.l.ws + a.l.o_part) + slot;
+        float* part = reinterpret_cast<float*>(a.l.ws + a.l.o_part + 4l * SLOTS) + (long)slot * TILE * TILE + threadIdx.x;
+        float* own = part + (long)slice * TILE * TILE;
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
-            for (int y = 0; y < NT; ++y) acc[x][y] += low[x][y];
+            for (int y = 0; y < NT; ++y)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    __hip_atomic_store(own + ((x * NT + y) * 16 + r) * 256, sum[x][y][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // Device-scope accesses go past the caches of the eight dies, and a wave's are complete when its count of outstanding ones
+        // is 0: the sums are in place before the arrival is counted.  (A release fence would write back a whole L2 per workgroup.)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (arrived != slices - 1) return;
+        if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);       // for the next launch
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int y = 0; y < NT; ++y) sum[x][y] = f32x16{};
+        for (int w = 0; w < slices; ++w)
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int y = 0; y < NT; ++y)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        sum[x][y][r] += __hip_atomic_load(part + (long)w * TILE * TILE + ((x * NT + y) * 16 + r) * 256, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     ksr_lds_barrier();                                  // LDS is free for the output tile
     // ---- values
-    const float* xis = reinterpret_cast<const float*>(ws + l.o_xi);
-    float* dv = reinterpret_cast<float*>(ws + l.o_d);
-    float* ev = reinterpret_cast<float*>(ws + l.o_e);
-    const Step& sp = a.p.s;
+    const float* xis = reinterpret_cast<const float*>(ws + of.xi);
+    float* dv = reinterpret_cast<float*>(ws + of.d);
+    float* ev = reinterpret_cast<float*>(ws + of.e);
+    const Step& sp = a.s;
     const float xi = xis[a.k], rn = KIND == X_NEXT ? 1.f / xis[a.k + 1] : 1.f;
-    int sub = 0;
-    const Mat& mat = find(a.p, l.base + (int)blockIdx.y, sub);
+    const Mat& mat = a.m[q];
     const Apply ap(sp, mat);
     const int mode = sp.muon ? MUON : sp.bf16 ? BF16 : F32;
 #pragma unroll
@@ -541,11 +708,11 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
 #pragma unroll
         for (int y = 0; y < NT; ++y)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row0 = ti * TILE + wr * W + 32 * x + 8 * q + 4 * (lane >> 5), c = tj * TILE + wc * W + 32 * y + (lane & 31);
+            for (int g = 0; g < 4; ++g) {
+                const int row0 = ti * TILE + wr * W + 32 * x + 8 * g + 4 * (lane >> 5), c = tj * TILE + wc * W + 32 * y + (lane & 31);
                 float v[4];
 #pragma unroll
-                for (int z = 0; z < 4; ++z) v[z] = acc[x][y][4 * q + z];
+                for (int z = 0; z < 4; ++z) v[z] = sum[x][y][4 * g + z];
                 if constexpr (KIND == A_OF_X) {
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
@@ -598,7 +765,7 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
                     }
                 }
 #pragma unroll
-                for (int z = 0; z < 4; ++z) acc[x][y][4 * q + z] = v[z];
+                for (int z = 0; z < 4; ++z) sum[x][y][4 * g + z] = v[z];
             }
     if constexpr (KIND == X_LAST) return;
     // ---- the tile and its transpose, hi and lo, through LDS: 16-byte stores of whole rows
@@ -607,10 +774,10 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
     long ld, ldt, plane;
     constexpr int planes = (KIND == X_NEXT || SPLIT) ? 2 : 1;
     if constexpr (KIND == X_NEXT) {
-        out = reinterpret_cast<_Float16*>(ws + l.o_x); outt = reinterpret_cast<_Float16*>(ws + l.o_xt[(a.k + 1) & 1]);
+        out = reinterpret_cast<_Float16*>(ws + of.x); outt = reinterpret_cast<_Float16*>(ws + of.xt(a.k + 1));
         ld = l.np; ldt = l.mp; plane = (long)l.mp * l.np;
     } else {
-        out = outt = reinterpret_cast<_Float16*>(ws + (KIND == A_OF_X ? l.o_r : l.o_b));
+        out = outt = reinterpret_cast<_Float16*>(ws + (KIND == A_OF_X ? of.r : of.b));
         ld = ldt = l.mp; plane = (long)l.mp * l.mp;
     }
 #pragma unroll
@@ -624,12 +791,12 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
 #pragma unroll
                 for (int y = 0; y < NT; ++y)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int r = wr * W + 32 * x + 8 * q + 4 * (lane >> 5), c = wc * W + 32 * y + (lane & 31);
+                    for (int g = 0; g < 4; ++g) {
+                        const int r = wr * W + 32 * x + 8 * g + 4 * (lane >> 5), c = wc * W + 32 * y + (lane & 31);
                         h4 w;
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            const float v = acc[x][y][4 * q + z];
+                            const float v = sum[x][y][4 * g + z];
                             const _Float16 hi = (_Float16)v;
                             w[z] = pl ? (_Float16)(v - (float)hi) : hi;
                         }
@@ -643,8 +810,8 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
             _Float16* o = (tr ? outt : out) + pl * plane;
             const long lo = tr ? ldt : ld;
             const int r0 = (tr ? tj : ti) * TILE, c0 = (tr ? ti : tj) * TILE;
-            for (int t = threadIdx.x; t < TILE * (TILE / 8); t += 256) {
-                const int r = t / (TILE / 8), c = t % (TILE / 8) * 8;
+            for (int w = threadIdx.x; w < TILE * (TILE / 8); w += 256) {
+                const int r = w / (TILE / 8), c = w % (TILE / 8) * 8;
                 *reinterpret_cast<uint4*>(o + (long)(r0 + r) * lo + c0 + c) = *reinterpret_cast<const uint4*>(stage + r * STG + c);
             }
             __syncthreads();
@@ -653,41 +820,64 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(GemmArgs a) {
 
 // ------------------------------------------------------------------------------------------------ host
 bool is_small(int rows, int cols) { return rows < cols ? rows <= 64 && cols <= 1024 : cols <= 64 && rows <= 1024; }
+bool empty(const KsrMatrix& q) { return !q.rows || !q.cols || !q.batch; }
 
-int tile_of(int m, int n) { return (long)((m + 127) / 128) * ((n + 127) / 128) >= 128 ? 128 : 64; }
+// Matrices that run together: as many as fit 1 GiB of buffers, at least one.  (entry, index in its batch) of the first one that
+// is left is advanced; returns the bytes the group needs, 0 at the end of the list.
+constexpr long WS_CAP = 1l << 30;
 
-long align256(long v) { return (v + 255) / 256 * 256; }
-
-void plan(Large& l, int rows, int cols, bool split) {
-    l = Large{};
-    l.tall = rows > cols;
-    l.m = l.tall ? cols : rows;
-    l.n = l.tall ? rows : cols;
-    const int tile = l.tile = tile_of(l.m, l.n);
-    l.mp = (l.m + tile - 1) / tile * tile;
-    l.np = (l.n + tile - 1) / tile * tile;
-    const long xp = 2l * l.mp * l.np, ap = 2l * l.mp * l.mp;
-    long o = 0;
-    l.o_x = o; o += align256(xp * (split ? 2 : 1));
-    l.o_xt[0] = o; o += align256(2 * xp);
-    l.o_xt[1] = o; o += align256(2 * xp);
-    l.o_r = o; o += align256(ap * (split ? 2 : 1));
-    l.o_b = o; o += align256(ap * (split ? 2 : 1));
-    l.o_d = o; o += align256(4l * l.mp);
-    l.o_e = o; o += align256(4l * l.mp);
-    l.o_xi = o; o += align256(4l * (MAX_STEPS + 1));
-    l.o_sq = o; o += align256(8l * NORM_PARTS);
-    l.per = o;
-}
-
-constexpr long WS_CAP = 1l << 30;           // matrices of one shape that run together: as many as fit 1 GiB, at least one
-constexpr int BATCH_CAP = 16384;
-
-long together(const Large& l, long count) {
-    long n = WS_CAP / l.per;
-    if (n < 1) n = 1;
-    if (n > BATCH_CAP) n = BATCH_CAP;
-    return n < count ? n : count;
+long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& sub, Large& l, Mat* m) {
+    const int entry0 = entry, sub0 = sub;
+    l.count = 0;
+    l.split = split;
+    for (int pass = 0; pass < 2; ++pass) {
+        // the tile: 128 where that gives at least 128 tiles of X (the wide tile's products run at 1.5 times the rate of the
+        // narrow one's; a chip that is half empty costs more)
+        l.tile = pass == 0 ? 128 : 64;
+        l.count = 0;
+        entry = entry0;
+        sub = sub0;
+        long off = 0;
+        int matrices = 0;
+        long sym = 0, full = 0;
+        for (; entry < count && l.count < MAX_LARGE; ++entry, sub = 0) {
+            const KsrMatrix& k = mats[entry];
+            if (empty(k) || is_small(k.rows, k.cols)) continue;
+            LMat& e = l.e[l.count];
+            e.tall = k.rows > k.cols;
+            e.m = e.tall ? k.cols : k.rows;
+            e.n = e.tall ? k.rows : k.cols;
+            e.mp = (e.m + l.tile - 1) / l.tile * l.tile;
+            e.np = (e.n + l.tile - 1) / l.tile * l.tile;
+            const long per = Offsets(e.mp, e.np, split).per, mt = e.mp / l.tile, nt = e.np / l.tile;
+            long room = (WS_CAP - off) / per;
+            if (room < 1) {
+                if (l.count) break;
+                room = 1;
+            }
+            if (room > 60000 - matrices) room = 60000 - matrices;               // the grid's second dimension
+            if (room < 1) break;
+            const int left = k.batch - sub;
+            e.nsub = left < room ? left : (int)room;
+            e.sub0 = sub;
+            const long elements = (long)e.m * e.n;
+            e.parts = elements / 8192 < 1 ? 1 : elements / 8192 < NORM_PARTS ? (int)(elements / 8192) : NORM_PARTS;
+            e.off = off;
+            e.first = matrices;
+            e.sym = (int)sym;
+            e.full = (int)full;
+            m[l.count++] = Mat{k.src, k.dst, k.momentum, (long)k.row_stride, (long)k.col_stride, (long)k.batch_stride, k.rows, k.cols, k.batch, 0};
+            off += e.nsub * per;
+            matrices += e.nsub;
+            sym += e.nsub * (mt * (mt + 1) / 2);
+            full += e.nsub * mt * nt;
+            if (e.nsub < left) { sub += e.nsub; break; }
+        }
+        if (!l.count) return 0;
+        l.o_part = off;
+        if (pass == 1 || full >= 128) break;
+    }
+    return l.o_part + 4l * SLOTS + 4l * SLOTS * l.tile * l.tile;
 }
 
 // Largest singular value that each step can reach from [0, 1], and that A and B stay inside f16's range
@@ -707,27 +897,47 @@ bool bounded(float a, float b, float c, int steps, float& gain) {
     return true;
 }
 
-template <int MODE, bool SPLIT> void start_large(const NormArgs& na, hipStream_t st) {
-    const Large& l = na.l;
-    hipLaunchKernelGGL((ns_norm_kernel<MODE>), dim3(NORM_PARTS, (unsigned)l.batch), dim3(256), 0, st, na);
-    hipLaunchKernelGGL((ns_prepare_kernel<MODE, SPLIT>), dim3((unsigned)(l.np / 64), (unsigned)(l.mp / 64), (unsigned)l.batch), dim3(256), 0, st, na);
+template <int MODE, bool SPLIT> void start_large(const LargeArgs& a, hipStream_t st) {
+    unsigned matrices = 0, parts = 1, tiles = 1;
+    for (int i = 0; i < a.l.count; ++i) {
+        const LMat& e = a.l.e[i];
+        matrices = (unsigned)(e.first + e.nsub);
+        if ((unsigned)e.parts > parts) parts = (unsigned)e.parts;
+        const unsigned t = (unsigned)((long)(e.mp / 64) * (e.np / 64));
+        if (t > tiles) tiles = t;
+    }
+    hipLaunchKernelGGL((ns_norm_kernel<MODE>), dim3(parts, matrices), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((ns_prepare_kernel<MODE, SPLIT>), dim3(tiles, matrices), dim3(256), 0, st, a);
 }
 
-template <int TILE, bool SPLIT> int run_large(const Mats& p, Large l, hipStream_t st) {
-    NormArgs na{p, l};
-    const int mode = mode_of(p.s);
-    if (mode == F32) start_large<F32, SPLIT>(na, st);
-    else if (mode == BF16) start_large<BF16, SPLIT>(na, st);
-    else start_large<MUON, SPLIT>(na, st);
+template <int TILE, bool SPLIT, int KIND> void product(LargeArgs& a, hipStream_t st) {
+    constexpr bool SYM = KIND == A_OF_X || KIND == B_OF_A;
+    const LMat& back = a.l.e[a.l.count - 1];
+    auto tiles_of = [](const LMat& e) { return e.nsub * (SYM ? e.mp / TILE * (e.mp / TILE + 1) / 2 : e.mp / TILE * (e.np / TILE)); };
+    const int tiles = (SYM ? back.sym : back.full) + tiles_of(back);
+    a.whole = tiles / CUS * CUS;
+    long cut = 0;                                       // workgroups if every chunk of the rest has one
+    for (int i = 0; i < a.l.count; ++i) {
+        const LMat& e = a.l.e[i];
+        const int first = SYM ? e.sym : e.full, from = a.whole > first ? a.whole : first, n = first + tiles_of(e) - from;
+        const int ch = chunk_of(KIND == A_OF_X ? e.n : e.m), kp = KIND == A_OF_X ? e.np : e.mp;
+        if (n > 0) cut += (long)n * ((kp + ch - 1) / ch);
+    }
+    a.cut = cut <= SLOTS;
+    hipLaunchKernelGGL((ns_gemm_kernel<TILE, SPLIT, KIND>), dim3((unsigned)(a.cut ? a.whole + cut : tiles)), dim3(256), 0, st, a);
+}
+
+template <int TILE, bool SPLIT> int run_large(LargeArgs& a, hipStream_t st) {
+    const int mode = mode_of(a.s);
+    if (mode == F32) start_large<F32, SPLIT>(a, st);
+    else if (mode == BF16) start_large<BF16, SPLIT>(a, st);
+    else start_large<MUON, SPLIT>(a, st);
     KSR_LAUNCH_CHECK("muon_batch");
-    const int mt = l.mp / TILE, nt = l.np / TILE;
-    const dim3 tri((unsigned)(mt * (mt + 1) / 2), (unsigned)l.batch), full((unsigned)(mt * nt), (unsigned)l.batch);
-    for (int k = 0; k < p.s.steps; ++k) {
-        GemmArgs g{p, l, k};
-        hipLaunchKernelGGL((ns_gemm_kernel<TILE, SPLIT, A_OF_X>), tri, dim3(256), 0, st, g);
-        hipLaunchKernelGGL((ns_gemm_kernel<TILE, SPLIT, B_OF_A>), tri, dim3(256), 0, st, g);
-        if (k + 1 < p.s.steps) hipLaunchKernelGGL((ns_gemm_kernel<TILE, SPLIT, X_NEXT>), full, dim3(256), 0, st, g);
-        else hipLaunchKernelGGL((ns_gemm_kernel<TILE, SPLIT, X_LAST>), full, dim3(256), 0, st, g);
+    for (a.k = 0; a.k < a.s.steps; ++a.k) {
+        product<TILE, SPLIT, A_OF_X>(a, st);
+        product<TILE, SPLIT, B_OF_A>(a, st);
+        if (a.k + 1 < a.s.steps) product<TILE, SPLIT, X_NEXT>(a, st);
+        else product<TILE, SPLIT, X_LAST>(a, st);
         KSR_LAUNCH_CHECK("muon_batch");
     }
     return KSR_OK;
@@ -749,8 +959,6 @@ int check_shapes(const KsrMatrix* mats, int count) {
     return KSR_OK;
 }
 
-bool empty(const KsrMatrix& q) { return !q.rows || !q.cols || !q.batch; }
-
 int check_mats(const KsrMatrix* mats, int count, int bf16, bool muon) {
     if (int rc = check_shapes(mats, count)) return rc;
     for (int i = 0; i < count; ++i) {
@@ -770,14 +978,10 @@ int check_mats(const KsrMatrix* mats, int count, int bf16, bool muon) {
 extern "C" int64_t ksr_muon_ws_bytes(const KsrMatrix* mats, int count, int split) {
     if (check_shapes(mats, count) != KSR_OK) return -1;
     int64_t most = 0;
-    for (int i = 0; i < count; ++i) {
-        if (empty(mats[i]) || is_small(mats[i].rows, mats[i].cols)) continue;
-        int64_t same = 0;                    // matrices of this shape in the list run together
-        for (int j = 0; j < count; ++j)
-            if (!empty(mats[j]) && mats[j].rows == mats[i].rows && mats[j].cols == mats[i].cols) same += mats[j].batch;
-        Large l;
-        plan(l, mats[i].rows, mats[i].cols, split != 0);
-        const int64_t need = together(l, same) * l.per;
+    Large l;
+    Mat m[MAX_LARGE];
+    for (int entry = 0, sub = 0; entry < count;) {
+        const int64_t need = next_group(mats, count, split != 0, entry, sub, l, m);
         if (need > most) most = need;
     }
     return most;
@@ -818,34 +1022,15 @@ extern "C" int ksr_muon_batch(const KsrMatrix* mats, int count, int bf16, int sp
         else hipLaunchKernelGGL(ns_small_kernel<MUON>, dim3((unsigned)total), dim3(512), 0, stream, p);
         KSR_LAUNCH_CHECK("muon_batch");
     }
-    // large ones: all of one shape together
-    for (int i = 0; i < count; ++i) {
-        if (empty(mats[i]) || small(mats[i])) continue;
-        bool seen = false;
-        for (int j = 0; j < i; ++j) seen = seen || (!empty(mats[j]) && mats[j].rows == mats[i].rows && mats[j].cols == mats[i].cols);
-        if (seen) continue;
-        Large l;
-        plan(l, mats[i].rows, mats[i].cols, split != 0);
-        l.ws = reinterpret_cast<char*>(ws);
-        for (int j = i; j < count;) {
-            p.count = 0;
-            int64_t total = 0;
-            for (; j < count && p.count < MAX_MATS; ++j) {
-                if (empty(mats[j]) || mats[j].rows != mats[i].rows || mats[j].cols != mats[i].cols) continue;
-                add(mats[j], (int)total);
-                total += mats[j].batch;
-            }
-            if (!p.count) break;
-            const long at_once = together(l, total);
-            for (int64_t base = 0; base < total; base += at_once) {
-                l.base = (int)base;
-                l.batch = (int)(total - base < at_once ? total - base : at_once);
-                int rc;
-                if (split) rc = l.tile == 128 ? run_large<128, true>(p, l, stream) : run_large<64, true>(p, l, stream);
-                else rc = l.tile == 128 ? run_large<128, false>(p, l, stream) : run_large<64, false>(p, l, stream);
-                if (rc) return rc;
-            }
-        }
+    LargeArgs g{};
+    g.s = p.s;
+    g.l.ws = reinterpret_cast<char*>(ws);
+    for (int entry = 0, sub = 0; entry < count;) {
+        if (!next_group(mats, count, split != 0, entry, sub, g.l, g.m)) break;
+        int rc;
+        if (split) rc = g.l.tile == 128 ? run_large<128, true>(g, stream) : run_large<64, true>(g, stream);
+        else rc = g.l.tile == 128 ? run_large<128, false>(g, stream) : run_large<64, false>(g, stream);
+        if (rc) return rc;
     }
     return KSR_OK;
 }
