@@ -36,7 +36,7 @@ struct Mat {
 
 struct Step {
     int steps, bf16, muon, nesterov;
-    float a, b, c, eps, gain;             // gain: most by which a step multiplies a singular value
+    float a, b, c, eps, log2_gain;        // gain: most by which a step multiplies a singular value
     float momentum, grad_scale, lr, wd, scale;
     const float* lr_dev;                  // replaces lr
 };
@@ -98,13 +98,15 @@ __device__ __forceinline__ float scales(const Step& s, double sumsq, int& e) {
     if (norm > 0) { (void)frexp(norm, &e); e = 15 - e; }
     return (float)(ldexp(1.0 / (norm + (double)s.eps), -e));
 }
-__device__ __forceinline__ float scale_of(const Step& s, double sumsq, int k) {
+// -log2 of the norm of X0, and from it xi[k], k > 0
+__device__ __forceinline__ double log_norm(const Step& s, double sumsq) {
     const double norm = sqrt(sumsq), nu = norm / (norm + (double)s.eps);
-    double lg = nu > 0 ? -log2(nu) - k * (double)log2f(s.gain) : 0.0;
-    lg = lg > 0 ? (lg < 100 ? floor(lg) : 100.0) : 0.0;
-    return (float)ldexp(1.0, -10 - (int)lg);
+    return nu > 0 ? -log2(nu) : 0.0;
 }
-
+__device__ __forceinline__ float scale_at(const Step& s, double lg, int k) {
+    const float f = (float)lg - (float)k * s.log2_gain;
+    return ldexpf(INV_S, -(int)(f > 0.f ? (f < 100.f ? floorf(f) : 100.f) : 0.f));      // NaN: 1
+}
 __device__ __forceinline__ float scaled(float u, int e) {       // u 2^e, also where 2^e is beyond a float's range
     return ldexpf(u, e);
 }
@@ -118,15 +120,16 @@ __device__ __forceinline__ double wave_sum(double v) {
 // ================================================================================================ small matrices
 // m <= 64, n <= 1024: one workgroup of eight waves per matrix runs the whole iteration.  X stays in registers: a wave owns NS
 // slabs of 32 columns in the accumulator layout of v_mfma_f32_32x32x16 (lane = column, register r = row 8 (r/4) + 4 (lane/32) +
-// r%4), which is the B operand's layout for the next product when both operands take k in that order.  Always SPLIT (the time
-// is latency).  LDS: partial sums of A per wave, R and B in hi and lo, one slab per wave on its way to X X^T.
+// r%4), which is the B operand's layout for the next product when both operands take k in that order.  Always SPLIT: the time
+// is latency (one wave or two per SIMD, three or four barriers a step), not matrix work.
+// The 64 x 64 matrices A and A^2 are four 32 x 32 tiles of four waves; both triangles are computed, so that a wave writes its
+// tile's transpose in 8-byte pieces and nothing else (symmetric up to the rounding of hi lo + lo hi).  For X X^T the slabs pass
+// through LDS, eight at a time, the upper four waves taking slabs 4 to 7 of them.
 constexpr int LD = 72;                                  // halves per row of R, B and a slab: 144 bytes
 
 struct SmallLds {
-    union {
-        float part[8][3 * 1024];                        // 96 KB: A's three 32 x 32 tiles per wave
-        _Float16 slab[8][2][32 * LD];                   // 72 KB: [column][row], hi and lo
-    };
+    _Float16 slab[8][2][32 * LD];                       // 72 KB: [column][row], hi and lo
+    float red[4][16][64];                               // 16 KB: the upper waves' sums
     _Float16 r[2][64 * LD], bm[2][64 * LD];             // 36 KB
     float d[64], ae[64];                                // diagonal of A; a + diagonal of B
     double sq[8];
@@ -136,12 +139,6 @@ __device__ __forceinline__ int acc_row(int r, int lane) { return 8 * (r >> 2) + 
 
 __device__ __forceinline__ f32x16 mfma(const h8& a, const h8& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-// (hi + lo)(hi + lo) without lo lo
-__device__ __forceinline__ f32x16 mfma3(const h8& ah, const h8& al, const h8& bh, const h8& bl, f32x16 c) {
-    c = mfma(al, bh, c);
-    c = mfma(ah, bl, c);
-    return mfma(ah, bh, c);
 }
 
 __device__ __forceinline__ h4 lds_tr4(const _Float16* p) {      // transposed read: see frag_of_slab
@@ -167,144 +164,183 @@ __device__ __forceinline__ h8 frag_row_acc(const _Float16* mat, int t, int s, in
     const h4 x = *reinterpret_cast<const h4*>(p), y = *reinterpret_cast<const h4*>(p + 8);
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-__device__ __forceinline__ void put2(_Float16 (&mat)[2][64 * LD], int r, int c, float v) {
-    const _Float16 hi = (_Float16)v;
-    mat[0][r * LD + c] = hi;
-    mat[1][r * LD + c] = (_Float16)(v - (float)hi);
+// four values as hi and lo to row j, columns i .. i + 3
+__device__ __forceinline__ void put4(_Float16 (&mat)[2][64 * LD], int j, int i, const float (&v)[4]) {
+    h4 hi, lo;
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+        hi[z] = (_Float16)v[z];
+        lo[z] = (_Float16)(v[z] - (float)hi[z]);
+    }
+    *reinterpret_cast<h4*>(&mat[0][j * LD + i]) = hi;
+    *reinterpret_cast<h4*>(&mat[1][j * LD + i]) = lo;
 }
 
 template <int MODE, int NS>
-__device__ __forceinline__ void small_body(const Mats& p, const Mat& mt, int sub, SmallLds& L) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
+__device__ __forceinline__ void small_body(const Step& st, const Mat& mt, int sub, SmallLds& L) {
+    const int lane0 = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool tall = mt.rows > mt.cols;
     const int m = tall ? mt.cols : mt.rows, n = tall ? mt.rows : mt.cols, slabs = (n + 31) >> 5;
-    // sum of squares, the momentum updated on the way; neighbouring threads along U's contiguous dimension
-    double sq = 0;
-    {
-        const bool by_col = mt.cs <= mt.rs;
-        const int inner = by_col ? mt.cols : mt.rows, total = mt.rows * mt.cols;
-        for (int t = threadIdx.x; t < total; t += 512) {
-            const int o = t / inner, i = t - o * inner;
-            const double u = load_u<MODE, true>(p.s, mt, sub, by_col ? o : i, by_col ? i : o);
-            sq = fma(u, u, sq);
-        }
-    }
-    sq = wave_sum(sq);
-    if (lane == 0) L.sq[wave] = sq;
-    __threadfence_block();
-    __syncthreads();
-    double total = 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) total += L.sq[w];
-    int e;
-    float xi = scales(p.s, total, e);
-    // slab s of this wave: columns 32 (wave + 8 s) ..
+    const Apply ap(st, mt);
+    // slab s of this wave: columns 32 (wave + 8 s) ..; all loads are in flight together
     h8 xh[NS][4], xl[NS][4];
+    float xi;
+    double lg;
+    {
+        const int lane = lane0, col = lane & 31;
+        float u[NS][32];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-        const int j = 32 * (wave + 8 * s) + col, jc = j < n ? j : n - 1;
+        for (int s = 0; s < NS; ++s) {
+            const int j = 32 * (wave + 8 * s) + col, jc = j < n ? j : n - 1;
+            float mo[MODE == MUON ? 32 : 1];
 #pragma unroll
-        for (int r = 0; r < 32; ++r) {
-            const int i = 32 * (r >> 4) + acc_row(r & 15, lane), ic = i < m ? i : m - 1;
-            const float u = load_u<MODE, false>(p.s, mt, sub, tall ? jc : ic, tall ? ic : jc);
-            const float v = i < m && j < n ? scaled(u, e) : 0.f;
-            const _Float16 hi = (_Float16)v;
-            xh[s][r >> 3][r & 7] = hi;
-            xl[s][r >> 3][r & 7] = (_Float16)(v - (float)hi);
-            if ((r & 7) == 7) __builtin_amdgcn_sched_barrier(0);      // eight loads in flight: more addresses would spill
+            for (int r = 0; r < 32; ++r) {
+                const int i = 32 * (r >> 4) + acc_row(r & 15, lane), ic = i < m ? i : m - 1;
+                const int row = tall ? jc : ic, c = tall ? ic : jc;
+                const long o = (long)sub * mt.bs + (long)row * mt.rs + (long)c * mt.cs;
+                if constexpr (MODE == BF16) u[s][r] = (float)reinterpret_cast<const __bf16*>(mt.src)[o];
+                else u[s][r] = reinterpret_cast<const float*>(mt.src)[o];
+                if constexpr (MODE == MUON) mo[r] = mt.mom[((long)sub * mt.rows + row) * mt.cols + c];
+            }
+            if constexpr (MODE == MUON) {               // every element has one lane; what a lane beyond the matrix read is dropped below
+#pragma unroll
+                for (int r = 0; r < 32; ++r) {
+                    const int i = 32 * (r >> 4) + acc_row(r & 15, lane);
+                    const float gs = u[s][r] * st.grad_scale, m1 = fmaf(st.momentum, mo[r], gs);
+                    if (i < m && j < n) mt.mom[((long)sub * mt.rows + (tall ? j : i)) * mt.cols + (tall ? i : j)] = m1;
+                    u[s][r] = st.nesterov ? fmaf(st.momentum, m1, gs) : m1;
+                }
+                if (NS > 1) __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        double sq = 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int j = 32 * (wave + 8 * s) + col;
+#pragma unroll
+            for (int r = 0; r < 32; ++r) {
+                const int i = 32 * (r >> 4) + acc_row(r & 15, lane);
+                if (!(i < m && j < n)) u[s][r] = 0.f;
+                sq = fma((double)u[s][r], (double)u[s][r], sq);
+            }
+        }
+        sq = wave_sum(sq);
+        if (lane == 0) L.sq[wave] = sq;
+        __syncthreads();
+        double total = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) total += L.sq[w];
+        int e;
+        xi = scales(st, total, e);
+        lg = log_norm(st, total);
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 32; ++r) {
+                const float v = scaled(u[s][r], e);
+                const _Float16 hi = (_Float16)v;
+                xh[s][r >> 3][r & 7] = hi;
+                xl[s][r >> 3][r & 7] = (_Float16)(v - (float)hi);
+            }
     }
-    const Apply ap(p.s, mt);
-    const int lane0 = lane;
-    for (int k = 0; k < p.s.steps; ++k) {
+    for (int k = 0; k < st.steps; ++k) {
         // an index the compiler cannot follow: it would otherwise keep every address and bound of the last step's stores (more
         // than 256 registers) through all steps
         int lane = lane0;
         asm volatile("" : "+v"(lane));
-        const int col = lane & 31;
-        // ---- A = X X^T: each wave over its own columns
-        f32x16 acc[3] = {};
+        const int col = lane & 31, half = lane >> 5, ti = (wave >> 1) & 1, tj = wave & 1;
+        // ---- A = X X^T
+        f32x16 acc = {}, low = {};
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
-            if (wave + 8 * s < slabs) {
+        for (int s = 0; s < NS; ++s) {
+            if (s) __syncthreads();                        // the slabs of the round before are read
 #pragma unroll
-                for (int pl = 0; pl < 2; ++pl)
+            for (int pl = 0; pl < 2; ++pl)
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {          // four rows 32 (q/4) + 8 (q%4) + 4 (lane/32) .. of the lane's column
-                        const h8& v = pl ? xl[s][q >> 1] : xh[s][q >> 1];
-                        const h4 w = (q & 1) ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3);
-                        *reinterpret_cast<h4*>(&L.slab[wave][pl][col * LD + 32 * (q >> 2) + 8 * (q & 3) + 4 * (lane >> 5)]) = w;
-                    }
-                asm volatile("" ::: "memory");             // a wave's LDS accesses are in order; its slab is its own
+                for (int q = 0; q < 8; ++q) {              // four rows 32 (q/4) + 8 (q%4) + 4 (lane/32) .. of the lane's column
+                    const h8& v = pl ? xl[s][q >> 1] : xh[s][q >> 1];
+                    const h4 w = (q & 1) ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3);
+                    *reinterpret_cast<h4*>(&L.slab[wave][pl][col * LD + 32 * (q >> 2) + 8 * (q & 3) + 4 * half]) = w;
+                }
+            __syncthreads();
+            const int first = 4 * (wave >> 2), left = slabs - 8 * s;
+            for (int w = first; w < first + 4 && w < left; ++w)
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
-                    h8 fh[2], fl[2];
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        fh[t] = frag_of_slab(L.slab[wave][0], t, ks, lane);
-                        fl[t] = frag_of_slab(L.slab[wave][1], t, ks, lane);
-                    }
-                    acc[0] = mfma3(fh[0], fl[0], fh[0], fl[0], acc[0]);
-                    acc[1] = mfma3(fh[1], fl[1], fh[0], fl[0], acc[1]);
-                    acc[2] = mfma3(fh[1], fl[1], fh[1], fl[1], acc[2]);
+                    const h8 ph = frag_of_slab(L.slab[w][0], ti, ks, lane), pl = frag_of_slab(L.slab[w][1], ti, ks, lane);
+                    const h8 qh = frag_of_slab(L.slab[w][0], tj, ks, lane), ql = frag_of_slab(L.slab[w][1], tj, ks, lane);
+                    acc = mfma(ph, qh, acc);
+                    low = mfma(ph, ql, low);
+                    low = mfma(pl, qh, low);
                 }
-                asm volatile("" ::: "memory");
-                __builtin_amdgcn_sched_barrier(0);
+        }
+        acc += low;
+        if (slabs > 4) {                                   // the upper waves' half
+            if (wave >= 4)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) L.red[wave - 4][r][lane] = acc[r];
+            __syncthreads();
+        }
+        if (wave < 4) {
+            if (slabs > 4)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[r] += L.red[wave][r][lane];
+            const float xi2 = xi * xi;
+            const int j = 32 * tj + col;
+            float dj = 0.f;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int i = 32 * ti + 8 * g + 4 * half;
+                float v[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    v[z] = acc[4 * g + z] * xi2;
+                    dj = i + z == j ? v[z] : dj;
+                    v[z] = i + z == j ? 0.f : v[z] * S;
+                }
+                put4(L.r, j, i, v);
             }
-        __syncthreads();                                   // slabs are read: their LDS becomes the partial sums'
-        if (wave < slabs)
-#pragma unroll
-            for (int t = 0; t < 3; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) L.part[wave][(t * 16 + r) * 64 + lane] = acc[t][r];
-        __syncthreads();
-        const int nw = slabs < 8 ? slabs : 8;
-        const float xi2 = xi * xi;
-#pragma unroll
-        for (int q = 0; q < 6; ++q) {
-            const int tr = wave + 8 * q, t = tr >> 4, r = tr & 15;
-            float v = 0.f;
-            for (int w = 0; w < nw; ++w) v += L.part[w][tr * 64 + lane];
-            v *= xi2;
-            const int i = (t > 0 ? 32 : 0) + acc_row(r, lane), j = (t > 1 ? 32 : 0) + col;
-            const bool diag = i == j;
-            if (diag) L.d[i] = v;
-            if (t == 1 || i >= j) {                        // the lower triangle decides both
-                const float w = diag ? 0.f : v * S;
-                put2(L.r, i, j, w);
-                if (!diag) put2(L.r, j, i, w);
-            }
+            if (ti == tj && ((col >> 2) & 1) == half) L.d[j] = dj;       // the lane that holds (j, j)
         }
         __syncthreads();
-        // ---- B = b A + c A^2, one 32 x 32 tile for each of three waves
-        if (wave < 3) {
-            const int ti = wave > 0 ? 1 : 0, tj = wave > 1 ? 1 : 0;
-            f32x16 g = {};
+        // ---- B = b A + c A^2; what multiplies X itself, a + diag B, already in the scales of the old and the new X
+        const bool last = k + 1 == st.steps;
+        const float xn = last ? 1.f : scale_at(st, lg, k + 1), rn = 1.f / xn;
+        if (wave < 4) {
+            f32x16 g0 = {}, g1 = {};
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-                g = mfma3(frag_row(L.r[0], ti, ks, lane), frag_row(L.r[1], ti, ks, lane), frag_row(L.r[0], tj, ks, lane),
-                          frag_row(L.r[1], tj, ks, lane), g);
+            for (int ks = 0; ks < 4; ++ks) {
+                const h8 ph = frag_row(L.r[0], ti, ks, lane), pl = frag_row(L.r[1], ti, ks, lane);
+                const h8 qh = frag_row(L.r[0], tj, ks, lane), ql = frag_row(L.r[1], tj, ks, lane);
+                g0 = mfma(ph, qh, g0);
+                g1 = mfma(ph, ql, g1);
+                g1 = mfma(pl, qh, g1);
+            }
+            g0 += g1;
             const int j = 32 * tj + col;
             const float dj = L.d[j];
+            float ej = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = 32 * ti + acc_row(r, lane);
-                const float di = L.d[i], sq2 = g[r] * (INV_S * INV_S);
-                if (i == j) {
-                    L.ae[i] = p.s.a + p.s.b * di + p.s.c * (di * di + sq2);
-                    put2(L.bm, i, i, 0.f);
-                } else if (i > j) {
-                    const float rij = ((float)L.r[0][i * LD + j] + (float)L.r[1][i * LD + j]) * INV_S;
-                    const float v = S * (p.s.b * rij + p.s.c * ((di + dj) * rij + sq2));
-                    put2(L.bm, i, j, v);
-                    put2(L.bm, j, i, v);
+            for (int g = 0; g < 4; ++g) {
+                const int i = 32 * ti + 8 * g + 4 * half;
+                const h4 rh = *reinterpret_cast<const h4*>(&L.r[0][j * LD + i]), rl = *reinterpret_cast<const h4*>(&L.r[1][j * LD + i]);
+                const float4 d4 = *reinterpret_cast<const float4*>(&L.d[i]);
+                const float di[4] = {d4.x, d4.y, d4.z, d4.w};
+                float v[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    const float rij = ((float)rh[z] + (float)rl[z]) * INV_S, sq2 = g0[4 * g + z] * (INV_S * INV_S);
+                    ej = i + z == j ? sq2 : ej;
+                    v[z] = i + z == j ? 0.f : S * (st.b * rij + st.c * ((di[z] + dj) * rij + sq2));
                 }
+                put4(L.bm, j, i, v);
             }
+            if (ti == tj && ((col >> 2) & 1) == half) L.ae[j] = (st.a + st.b * dj + st.c * (dj * dj + ej)) * (xi * rn);
         }
         __syncthreads();
-        // ---- X <- (a + diag B) X + B X
-        const float xn = k + 1 < p.s.steps ? scale_of(p.s, total, k + 1) : 1.f, rn = 1.f / xn, alpha = xi * INV_S;
-        const bool last = k + 1 == p.s.steps;
+        // ---- X <- (a + diag B) X + B X.  The products with a lo part go into the accumulators before those of the hi parts: the
+        // large sum is rounded four times, not twelve.  fmaf on f16 values is one mixed-precision instruction.
+        const float alpha = xi * rn * INV_S;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
             if (wave + 8 * s < slabs) {
@@ -312,24 +348,41 @@ __device__ __forceinline__ void small_body(const Mats& p, const Mat& mt, int sub
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        x[t] = mfma3(frag_row_acc(L.bm[0], t, ks, lane), frag_row_acc(L.bm[1], t, ks, lane), xh[s][ks], xl[s][ks], x[t]);
-                const int j = 32 * (wave + 8 * s) + col;
-#pragma unroll
-                for (int r = 0; r < 32; ++r) {
-                    const int i = 32 * (r >> 4) + acc_row(r & 15, lane);
-                    const float old = ((float)xh[s][r >> 3][r & 7] + (float)xl[s][r >> 3][r & 7]) * xi;
-                    const float v = fmaf(L.ae[i], old, x[r >> 4][r & 15] * alpha);
-                    if (last) {
-                        if (i < m && j < n) ap.store<MODE>(mt, ((long)sub * mt.rows + (tall ? j : i)) * mt.cols + (tall ? i : j), v);
-                    } else {
-                        const float w = v * rn;
-                        const _Float16 hi = (_Float16)w;
-                        xh[s][r >> 3][r & 7] = hi;
-                        xl[s][r >> 3][r & 7] = (_Float16)(w - (float)hi);
+                    for (int t = 0; t < 2; ++t) {
+                        x[t] = mfma(frag_row_acc(L.bm[0], t, ks, lane), xl[s][ks], x[t]);
+                        x[t] = mfma(frag_row_acc(L.bm[1], t, ks, lane), xh[s][ks], x[t]);
                     }
-                    if ((r & 7) == 7) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) x[t] = mfma(frag_row_acc(L.bm[0], t, ks, lane), xh[s][ks], x[t]);
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    const float4 e4 = *reinterpret_cast<const float4*>(&L.ae[32 * (g >> 2) + 8 * (g & 3) + 4 * half]);
+                    const float ae[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const int r = 4 * g + z;
+                        x[g >> 2][r & 15] = fmaf((float)xh[s][r >> 3][r & 7], ae[z], fmaf((float)xl[s][r >> 3][r & 7], ae[z], x[g >> 2][r & 15] * alpha));
+                    }
                 }
+                if (last) {
+                    const int j = 32 * (wave + 8 * s) + col;
+#pragma unroll
+                    for (int r = 0; r < 32; ++r) {
+                        const int i = 32 * (r >> 4) + acc_row(r & 15, lane);
+                        if (i < m && j < n) ap.store<MODE>(mt, ((long)sub * mt.rows + (tall ? j : i)) * mt.cols + (tall ? i : j), x[r >> 4][r & 15]);
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 32; ++r) {
+                        const float v = x[r >> 4][r & 15];
+                        const _Float16 hi = (_Float16)v;
+                        xh[s][r >> 3][r & 7] = hi;
+                        xl[s][r >> 3][r & 7] = (_Float16)fmaf((float)hi, -1.f, v);
+                    }
+                }
+                if (NS > 1) __builtin_amdgcn_sched_barrier(0);
             }
         xi = xn;
     }
@@ -341,9 +394,9 @@ __global__ void __launch_bounds__(512) ns_small_kernel(Mats p) {
     int sub;
     const Mat& mt = find(p, (int)blockIdx.x, sub);
     const int n = mt.rows > mt.cols ? mt.rows : mt.cols;
-    if (n <= 256) small_body<MODE, 1>(p, mt, sub, L);
-    else if (n <= 512) small_body<MODE, 2>(p, mt, sub, L);
-    else small_body<MODE, 4>(p, mt, sub, L);
+    if (n <= 256) small_body<MODE, 1>(p.s, mt, sub, L);
+    else if (n <= 512) small_body<MODE, 2>(p.s, mt, sub, L);
+    else small_body<MODE, 4>(p.s, mt, sub, L);
 }
 
 // ================================================================================================ large matrices
@@ -483,7 +536,7 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
     int e;
     const float xi0 = scales(a.s, total, e);
     if (blockIdx.x == 0 && (int)threadIdx.x <= a.s.steps)
-        reinterpret_cast<float*>(ws + of.xi)[threadIdx.x] = threadIdx.x == 0 ? xi0 : scale_of(a.s, total, threadIdx.x);
+        reinterpret_cast<float*>(ws + of.xi)[threadIdx.x] = threadIdx.x == 0 ? xi0 : scale_at(a.s, log_norm(a.s, total), (int)threadIdx.x);
     const int i0 = (int)blockIdx.x / nj * 64, j0 = (int)blockIdx.x % nj * 64;
     const bool across = (mt.cs <= mt.rs) != (le.tall != 0);             // whether columns of X are contiguous in U
     for (int t = threadIdx.x; t < 4096; t += 256) {
@@ -881,7 +934,7 @@ long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& s
 }
 
 // Largest singular value that each step can reach from [0, 1], and that A and B stay inside f16's range
-bool bounded(float a, float b, float c, int steps, float& gain) {
+bool bounded(float a, float b, float c, int steps, float& log2_gain) {
     double top = 1.0, g = fabs((double)a);
     for (int k = 0; k < steps; ++k) {
         double next = 0;
@@ -893,7 +946,7 @@ bool bounded(float a, float b, float c, int steps, float& gain) {
         }
         top = next;
     }
-    gain = (float)(g > 1 ? g : 1);
+    log2_gain = (float)(g > 1 ? log2(g) : 0);
     return true;
 }
 
@@ -995,8 +1048,8 @@ extern "C" int ksr_muon_batch(const KsrMatrix* mats, int count, int bf16, int sp
     KSR_CHECK_ARG(steps >= 1 && steps <= MAX_STEPS, "muon_batch: %d steps (1 to %d)", steps, MAX_STEPS);
     KSR_CHECK_ARG(eps >= 0.f && eps < INFINITY, "muon_batch: eps = %g", (double)eps);
     Mats p{};
-    p.s = Step{steps, bf16, muon, nesterov, a, b, c, eps, 1.f, momentum, grad_scale, lr, weight_decay, scale, lr_dev};
-    KSR_UNSUPPORTED(!bounded(a, b, c, steps, p.s.gain), "muon_batch: with coefficients (%g, %g, %g) %d steps leave the range of the products (30)",
+    p.s = Step{steps, bf16, muon, nesterov, a, b, c, eps, 0.f, momentum, grad_scale, lr, weight_decay, scale, lr_dev};
+    KSR_UNSUPPORTED(!bounded(a, b, c, steps, p.s.log2_gain), "muon_batch: with coefficients (%g, %g, %g) %d steps leave the range of the products (30)",
                     (double)a, (double)b, (double)c, steps);
     KSR_CHECK_ARG(ws_bytes >= ksr_muon_ws_bytes(mats, count, split), "muon_batch: the workspace has %lld bytes, %lld are needed",
                   (long long)ws_bytes, (long long)ksr_muon_ws_bytes(mats, count, split));

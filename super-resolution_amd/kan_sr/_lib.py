@@ -84,6 +84,12 @@ def _declare(L: ctypes.CDLL) -> None:
     L.ksr_tx_bwd_wg_slab_floats.restype = c_int64
     L.ksr_group_norm_ws_floats.restype = c_int64
     L.ksr_muon_ws_bytes.restype = c_int64
+    # argument types where a call's time is the host's: plain Python numbers are converted without wrapper objects
+    L.ksr_group_norm_ws_floats.argtypes = [c_int64, c_int64, c_int, c_int, c_int]
+    L.ksr_group_norm_fwd.argtypes = [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p]
+    L.ksr_group_norm_bwd.argtypes = [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64] + [c_void_p] * 7 + [c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]
+    L.ksr_muon_ws_bytes.argtypes = [c_void_p, c_int, c_int]
+    L.ksr_muon_batch.argtypes = [c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_float, c_float, c_float, c_int, c_float, c_float, c_void_p, c_float, c_float, c_void_p, c_int64, c_void_p]
 
 
 # every symbol include/ksr.h declares (tests/test_host_logic.py compares the two lists)

@@ -7,8 +7,7 @@ is all this package's hyper-encoders have, run in one launch for the whole list.
 """
 from __future__ import annotations
 
-import ctypes
-from ctypes import byref, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import c_int64
 from typing import Iterable, Optional, Sequence
 
 import torch
@@ -16,27 +15,29 @@ import torch
 from ._lib import KsrError, check, lib, on_device_of, stream
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+MATRIX_WORDS = 8                                  # KsrMatrix of include/ksr.h as 64-bit words
 
 
-class _Matrix(ctypes.Structure):                  # KsrMatrix of include/ksr.h
-    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("momentum", c_void_p), ("row_stride", c_int64), ("col_stride", c_int64),
-                ("batch_stride", c_int64), ("rows", c_int32), ("cols", c_int32), ("batch", c_int32), ("reserved", c_int32)]
+def _matrix(src: int, dst: int, momentum: int, row_stride: int, col_stride: int, batch_stride: int, rows: int, cols: int,
+            batch: int) -> tuple:
+    """One KsrMatrix: three addresses, three strides, rows | cols and batch | 0 as pairs of 32 bits."""
+    return src, dst, momentum, row_stride, col_stride, batch_stride, rows | cols << 32, batch
 
 
-def _run(mats, device_of: torch.Tensor, bf16: bool, split: bool, steps: int, coefficients, eps: float, muon: bool = False,
+def _run(words: list, device_of: torch.Tensor, bf16: bool, split: bool, steps: int, coefficients, eps: float, muon: bool = False,
          momentum: float = 0.0, nesterov: bool = False, grad_scale: float = 1.0, lr: float = 0.0,
          lr_dev: Optional[torch.Tensor] = None, weight_decay: float = 0.0, scale: float = 0.0) -> None:
     L = lib()
-    n = c_int(len(mats))
+    mats, n = (c_int64 * len(words))(*words), len(words) // MATRIX_WORDS
     with on_device_of(device_of):
-        nbytes = int(L.ksr_muon_ws_bytes(mats, n, c_int(split)))
-        check(min(nbytes, 0), "ksr_muon_ws_bytes")
+        nbytes = L.ksr_muon_ws_bytes(mats, n, split)
+        if nbytes < 0:
+            check(int(nbytes), "ksr_muon_ws_bytes")
         ws = torch.empty(nbytes, device=device_of.device, dtype=torch.uint8) if nbytes else None
         a, b, c = coefficients
-        check(L.ksr_muon_batch(mats, n, c_int(bf16), c_int(split), c_int(muon), c_int(steps), c_float(a), c_float(b), c_float(c),
-                               c_float(eps), c_float(momentum), c_int(nesterov), c_float(grad_scale), c_float(lr),
-                               c_void_p(lr_dev.data_ptr() if lr_dev is not None else 0), c_float(weight_decay), c_float(scale),
-                               c_void_p(ws.data_ptr() if nbytes else 0), c_int64(nbytes), stream()), "ksr_muon_batch")
+        check(L.ksr_muon_batch(mats, n, bf16, split, muon, steps, a, b, c, eps, momentum, nesterov, grad_scale, lr,
+                               lr_dev.data_ptr() if lr_dev is not None else None, weight_decay, scale,
+                               ws.data_ptr() if nbytes else None, nbytes, stream()), "ksr_muon_batch")
 
 
 def _steps_and_coefficients(steps, coefficients):
@@ -77,9 +78,9 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
     u = u.unsqueeze(0) if u.dim() == 2 else u.reshape(-1, *u.shape[-2:])
     if max(u.shape) > 1 << 24:
         raise KsrError(f"newton_schulz: {tuple(g.shape)} is too large")
-    mats = (_Matrix * 1)()
-    mats[0] = (u.data_ptr(), out.data_ptr(), None, u.stride(1), u.stride(2), u.stride(0), u.shape[1], u.shape[2], u.shape[0], 0)
-    _run(mats, g, g.dtype is torch.bfloat16, split, steps, coefficients, eps)
+    batch, rows, cols = u.shape
+    bs, rs, cs = u.stride()
+    _run(_matrix(u.data_ptr(), out.data_ptr(), 0, rs, cs, bs, rows, cols, batch), g, g.dtype is torch.bfloat16, split, steps, coefficients, eps)
     return out
 
 
@@ -116,28 +117,31 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
     f32 = torch.float32
     if lr_dev is not None and (lr_dev.dtype is not f32 or lr_dev.numel() != 1 or lr_dev.device != device):
         raise KsrError("muon_update: lr_dev must be one float32 on the weights' device")
-    mats = (_Matrix * len(weights))()
-    held, seen = [], set()
+    words, held, seen = [], [], set()
     for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
         shape = as_matrix(w.shape)
         if shape is None:
             raise KsrError(f"muon_update: tensor {i} is {tuple(w.shape)}: matrices only (vectors belong to Adam)")
-        if max(shape) > 1 << 24:
+        rows, cols = shape
+        if rows > 1 << 24 or cols > 1 << 24:
             raise KsrError(f"muon_update: tensor {i}: {tuple(w.shape)} is too large")
         if not (w.dtype is g.dtype is m.dtype is f32) or w.device != device or g.device != device or m.device != device:
             raise KsrError(f"muon_update: tensor {i}: weight, gradient and momentum must be float32 on {device}")
         if g.shape != w.shape or m.shape != w.shape or not w.is_contiguous() or not m.is_contiguous():
             raise KsrError(f"muon_update: tensor {i}: gradient and momentum must have the weight's shape {tuple(w.shape)}, weight "
                            "and momentum be contiguous")
-        if g.dim() > 2 or g.layout is not torch.strided:
-            g = g.contiguous().view(shape)
+        if g.dim() == 2:
+            rs, cs = g.stride()
+        else:
+            g, rs, cs = g.contiguous(), cols, 1
             held.append(g)
         wp, mp = w.data_ptr(), m.data_ptr()
-        if w.numel() and (wp in seen or mp in seen or wp == mp):
+        if wp and (wp in seen or mp in seen or wp == mp):
             raise KsrError(f"muon_update: tensor {i}'s weight or momentum is in the list twice")
-        seen.update((wp, mp))
-        mats[i] = (g.data_ptr(), wp, mp, g.stride(0), g.stride(1), 0, shape[0], shape[1], 1, 0)
-    _run(mats, weights[0], False, _split(precision, f32), steps, coefficients, eps, True, momentum, nesterov, grad_scale, lr,
+        seen.add(wp)
+        seen.add(mp)
+        words += _matrix(g.data_ptr(), wp, mp, rs, cs, 0, rows, cols, 1)
+    _run(words, weights[0], False, _split(precision, f32), steps, coefficients, eps, True, momentum, nesterov, grad_scale, lr,
          lr_dev, weight_decay, scale)
     # the kernels write behind torch's back: whoever keys on the version counters (autograd, the UNet's kernel-layout weights) sees it
     torch.autograd.graph.increment_version(weights + momenta)

@@ -5,7 +5,7 @@ forward and backward below is one or more hand-written HIP kernels.
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_int64, c_void_p
+from ctypes import c_int, c_int64
 from typing import Optional, Sequence
 
 import torch
@@ -216,23 +216,33 @@ def _pixel_rows(t: torch.Tensor):
     return t, t.stride(0) if B > 1 else 0, step if step is not None else 0, S
 
 
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _group_norm_fwd(x, weight, bias, groups, eps, act):
+    """-> (y, x as it was read, statistics, (image stride, pixel stride, pixels))."""
+    x, xb, xp, S = _pixel_rows(x)
+    B, C = x.shape[0], x.shape[-1]
+    L = lib()
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    with on_device_of(x):
+        n = L.ksr_group_norm_ws_floats(B, S, C, groups, 0)
+        if n < 0:
+            check(int(n), "ksr_group_norm_ws_floats")
+        stats = torch.empty(2 * B * groups, device=x.device, dtype=torch.float32)
+        ws = torch.empty(n, device=x.device, dtype=torch.float32)
+        check(L.ksr_group_norm_fwd(x.data_ptr(), xb, xp, _address(weight), _address(bias), y.data_ptr(), stats.data_ptr(),
+                                   ws.data_ptr(), B, S, C, groups, eps, act, x.dtype is torch.bfloat16, stream()), "ksr_group_norm_fwd")
+    return y, x, stats, (xb, xp, S)
+
+
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        x, xb, xp, S = _pixel_rows(x)
-        B, C = x.shape[0], x.shape[-1]
-        bf16 = x.dtype is torch.bfloat16
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        stats = torch.empty(B, groups, 2, device=x.device, dtype=torch.float32)
-        with on_device_of(x):
-            n = int(lib().ksr_group_norm_ws_floats(c_int64(B), c_int64(S), c_int(C), c_int(groups), c_int(0)))
-            check(min(n, 0), "ksr_group_norm_ws_floats")
-            ws = torch.empty(n, device=x.device, dtype=torch.float32)
-            check(lib().ksr_group_norm_fwd(c_void_p(x.data_ptr()), c_int64(xb), c_int64(xp), ptr(weight), ptr(bias), ptr(y),
-                                           ptr(stats), ptr(ws), c_int64(B), c_int64(S), c_int(C), c_int(groups), c_float(eps),
-                                           c_int(act), c_int(bf16), stream()), "ksr_group_norm_fwd")
+        y, x, stats, layout = _group_norm_fwd(x, weight, bias, groups, eps, act)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.cfg = (groups, act, xb, xp, S)
+        ctx.cfg = (groups, act) + layout
         return y
 
     @staticmethod
@@ -241,19 +251,17 @@ class _GroupNormAct(torch.autograd.Function):
         x, weight, bias, stats = ctx.saved_tensors
         groups, act, xb, xp, S = ctx.cfg
         B, C = x.shape[0], x.shape[-1]
-        dy, db_, dp, _ = _pixel_rows(dy)
+        dy, gb, gp, _ = _pixel_rows(dy)
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        L = lib()
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_x else None
         dw = torch.empty(C, device=x.device, dtype=torch.float32) if want_w else None
         db = torch.empty(C, device=x.device, dtype=torch.float32) if want_b else None
         with on_device_of(x):
-            n = int(lib().ksr_group_norm_ws_floats(c_int64(B), c_int64(S), c_int(C), c_int(groups), c_int(1)))
-            check(min(n, 0), "ksr_group_norm_ws_floats")
-            ws = torch.empty(n, device=x.device, dtype=torch.float32)
-            check(lib().ksr_group_norm_bwd(c_void_p(x.data_ptr()), c_int64(xb), c_int64(xp), c_void_p(dy.data_ptr()),
-                                           c_int64(db_), c_int64(dp), ptr(weight), ptr(bias), ptr(stats), ptr(dx), ptr(dw), ptr(db),
-                                           ptr(ws), c_int64(B), c_int64(S), c_int(C), c_int(groups), c_int(act),
-                                           c_int(x.dtype is torch.bfloat16), stream()), "ksr_group_norm_bwd")
+            ws = torch.empty(L.ksr_group_norm_ws_floats(B, S, C, groups, 1), device=x.device, dtype=torch.float32)
+            check(L.ksr_group_norm_bwd(x.data_ptr(), xb, xp, dy.data_ptr(), gb, gp, _address(weight), _address(bias), stats.data_ptr(),
+                                       _address(dx), _address(dw), _address(db), ws.data_ptr(), B, S, C, groups, act,
+                                       x.dtype is torch.bfloat16, stream()), "ksr_group_norm_bwd")
         return dx, dw, db, None, None, None
 
 
@@ -284,4 +292,6 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
             raise KsrError(f"group_norm_act: {name} must be float32 [{C}] on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    return _GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation])
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation])
+    return _group_norm_fwd(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation])[0]

@@ -72,14 +72,12 @@ def test_muon_refuses_what_it_cannot_take():
 
 def test_muon_refuses_at_the_abi():
     from kan_sr import _lib
-    from kan_sr.muon import _Matrix
+    from kan_sr.muon import MATRIX_WORDS, _matrix
     L = _lib.lib()
     A = 1 << 20                                  # addresses that are never read: the checks come first
 
     def one(src=A, dst=A, mom=A, rs=8, rows=8, cols=8, batch=1):
-        m = (_Matrix * 1)()
-        m[0] = (src, dst, mom, rs, 1, 0, rows, cols, batch, 0)
-        return m
+        return (c_int64 * MATRIX_WORDS)(*_matrix(src or 0, dst or 0, mom or 0, rs, 1, 0, rows & 0xffffffff, cols, batch))
 
     def call(mats, bf16=0, muon=1, steps=5, coef=(3.4445, -4.775, 2.0315), eps=1e-7, ws=None, ws_bytes=0, count=1):
         return L.ksr_muon_batch(mats, c_int(count), c_int(bf16), c_int(1), c_int(muon), c_int(steps), *(c_float(v) for v in coef),
