@@ -11,72 +11,11 @@
 //   M2 = M2a + M2b + d^2 na nb / (na + nb):
 // E[x^2] - mu^2 would lose everything where |mu| >> sigma.  fp32 throughout.  Every sum has a fixed order: results do not
 // change from run to run.
-#include "ksr_common.h"
+#include "ksr_group_norm.h"
 
 namespace {
 
 constexpr int THREADS = 256;
-
-struct GnArgs {
-    const void* x; const void* dy; void* out;          // out: y (forward) or dx (backward), dense
-    const float* w; const float* b;                    // [C] or null
-    float* stats;                                      // [B][G][2]: mean, 1 / sqrt(var + eps)
-    float* part;                                       // per-chunk partial results
-    float* coef;                                       // backward: [B][G][2] mean(w dz), mean(w dz xhat)
-    float* chsum;                                      // backward: [B][2][C] sum dz, sum dz xhat
-    float* dw; float* db;
-    long xs_b, xs_p, ds_b, ds_p;                       // image and pixel strides of x, dy in elements
-    long B, S, chunk, nchunk;
-    int C, G, Cg, CB, nblk, GB, CV, PL;                // channels per block, blocks, group slots per block, vectors, pixel lanes
-    float eps;
-};
-
-template <int BYTES> struct RawOf;
-template <> struct RawOf<16> { typedef ksr_u32x4_t T; };
-template <> struct RawOf<8> { typedef unsigned T __attribute__((ext_vector_type(2))); };
-template <> struct RawOf<4> { typedef unsigned T; };
-template <> struct RawOf<2> { typedef unsigned short T; };
-
-template <class T, int VEC> struct Vec {
-    typedef typename RawOf<sizeof(T) * VEC>::T Raw;
-    static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[VEC]) {
-        T t[VEC];
-        __builtin_memcpy(t, &r, sizeof(r));
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = (float)t[i];
-    }
-    static __device__ __forceinline__ Raw pack(const float (&v)[VEC]) {      // bf16: rounded to nearest even, once
-        T t[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) t[i] = (T)v[i];
-        Raw r;
-        __builtin_memcpy(&r, t, sizeof(r));
-        return r;
-    }
-};
-
-template <int ACT> __device__ __forceinline__ float act_of(float z) {
-    if constexpr (ACT == KSR_ACT_RELU) return z < 0.f ? 0.f : z;                // NaN stays NaN
-    else if constexpr (ACT == KSR_ACT_SILU) return z * ksr_sigmoid(z);
-    else if constexpr (ACT == KSR_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    else return z;
-}
-template <int ACT> __device__ __forceinline__ float act_slope(float z) {
-    if constexpr (ACT == KSR_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-    else if constexpr (ACT == KSR_ACT_SILU) {
-        const float s = ksr_sigmoid(z);
-        return s * (1.f + z * (1.f - s));
-    } else if constexpr (ACT == KSR_ACT_GELU)
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
-               z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
-    else return 1.f;
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-    return v;
-}
 
 // Where this workgroup and thread work: blockIdx.x = (image * nblk + channel block) * nchunk + chunk.
 template <int VEC> struct Place {
@@ -103,14 +42,23 @@ template <int VEC> struct Place {
     }
 };
 
+template <class V, class T> __device__ __forceinline__ typename V::Raw ld(const T* p) { return *reinterpret_cast<const typename V::Raw*>(p); }
+// Results past the caches where they are large: the pass that writes them reads x (and dy) a second time, and what of it the
+// caches still hold stays there (4 x 512 x 512 x 128 bf16: 161 instead of 180 us).  Smaller results are left to whoever reads next.
+template <class V, bool PAST, class T> __device__ __forceinline__ void put(T* p, const typename V::Raw& v) {
+    if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<typename V::Raw*>(p));
+    else *reinterpret_cast<typename V::Raw*>(p) = v;
+}
+
 // vectors in flight per thread: 64 bytes of 16-byte loads, eight of the narrower ones
 template <class T, int VEC> constexpr int in_flight() { return sizeof(T) * VEC == 16 ? 4 : 8; }
 
 // ------------------------------------------------------------------------------------------------ statistics
-// ONE: a vector's channels belong to one group (Cg % VEC == 0): one (mean, M2) per thread instead of one per channel.
-template <class T, int VEC, bool ONE>
+// NE: entries (mean, M2) of a thread, each over VEC / NE channels of one group: 1 where a vector lies in one group, VEC / Cg where
+// it holds whole ones, VEC otherwise.
+template <class T, int VEC, int NE>
 __global__ void __launch_bounds__(THREADS) gn_stats_kernel(GnArgs a) {
-    constexpr int NE = ONE ? 1 : VEC, R = in_flight<T, VEC>();
+    constexpr int PE = VEC / NE, R = in_flight<T, VEC>();
     typedef Vec<T, VEC> V;
     __shared__ float smean[THREADS * NE], sm2[THREADS * NE], sn[THREADS];
     const Place<VEC> w(a, blockIdx.x);
@@ -119,36 +67,38 @@ __global__ void __launch_bounds__(THREADS) gn_stats_kernel(GnArgs a) {
     for (int i = 0; i < NE; ++i) mean[i] = m2[i] = 0.f;
     if (w.active) {
         const T* src = reinterpret_cast<const T*>(a.x) + w.b * a.xs_b + w.c0 + w.tv * VEC;
+        typename V::Raw next[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) next[r] = ld<V>(src + w.pixel(w.p0 + w.pl, r, a.PL) * a.xs_p);
         for (long base = w.p0 + w.pl; base < w.p1; base += (long)R * a.PL) {
-            typename V::Raw raw[R];
+            float v[R][VEC], s[NE], q[NE];
             int cnt = 0;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                raw[r] = *reinterpret_cast<const typename V::Raw*>(src + w.pixel(base, r, a.PL) * a.xs_p);
-                cnt += base + (long)r * a.PL < w.p1;
-            }
-            float v[R][VEC], s[NE], q[NE];
+                V::unpack(next[r], v[r]);
+                const bool ok = base + (long)r * a.PL < w.p1;
+                cnt += ok;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                V::unpack(raw[r], v[r]);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) v[r][i] = r < cnt ? v[r][i] : 0.f;
+                for (int i = 0; i < VEC; ++i) v[r][i] = ok ? v[r][i] : 0.f;
             }
+            // the next tile is on its way while this one is summed
+#pragma unroll
+            for (int r = 0; r < R; ++r) next[r] = ld<V>(src + w.pixel(base + (long)R * a.PL, r, a.PL) * a.xs_p);
 #pragma unroll
             for (int i = 0; i < NE; ++i) s[i] = q[i] = 0.f;
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) s[ONE ? 0 : i] += v[r][i];
-            const float nt = (float)(cnt * (ONE ? VEC : 1)), rn = 1.f / nt;
+                for (int i = 0; i < VEC; ++i) s[i / PE] += v[r][i];
+            const float nt = (float)(cnt * PE), rn = 1.f / nt;
 #pragma unroll
             for (int i = 0; i < NE; ++i) s[i] *= rn;                     // the tile's mean
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float d = r < cnt ? v[r][i] - s[ONE ? 0 : i] : 0.f;
-                    q[ONE ? 0 : i] = fmaf(d, d, q[ONE ? 0 : i]);
+                    const float d = r < cnt ? v[r][i] - s[i / PE] : 0.f;
+                    q[i / PE] = fmaf(d, d, q[i / PE]);
                 }
             const float f = nt / (n + nt);
 #pragma unroll
@@ -171,7 +121,7 @@ __global__ void __launch_bounds__(THREADS) gn_stats_kernel(GnArgs a) {
     }
     __syncthreads();
     // a wave per group that this channel block touches: join the entries of its channels and the pixel lanes
-    const int lane = threadIdx.x & 63, per = ONE ? VEC : 1;
+    const int lane = threadIdx.x & 63, per = PE;
     const int g0 = w.c0 / a.Cg, g1 = (w.c0 + w.cb - 1) / a.Cg;
     for (int g = g0 + ((int)threadIdx.x >> 6); g <= g1; g += THREADS / 64) {
         const int lo = (g * a.Cg > w.c0 ? g * a.Cg - w.c0 : 0) / per;
@@ -228,13 +178,48 @@ __global__ void __launch_bounds__(THREADS) gn_stats_join_kernel(GnArgs a) {
     }
 }
 
-// the thread's channels: mean, rstd of their groups, weight and bias
+// The same inside the pass that uses it, where an image has few chunks: all groups of the image (G <= 256, one channel block) to
+// st, 256 / 2^k lanes per group; saves a launch.
+__device__ __forceinline__ void join_stats(const GnArgs& a, long b, float2* st, float (*lds)[3]) {
+    int tg = 1;
+    while (tg < a.G) tg *= 2;
+    const int t = threadIdx.x, g = t & (tg - 1), k0 = t / tg, kl = THREADS / tg;
+    float n = 0.f, m = 0.f, q = 0.f;
+    if (g < a.G)
+#pragma unroll 4
+        for (int c = k0; c < (int)a.nchunk; c += kl) {
+            const float2 p = *reinterpret_cast<const float2*>(a.part + 2 * ((b * a.nchunk + c) * a.GB + g));
+            const long left = a.S - c * a.chunk;
+            const float nc = (float)(left < a.chunk ? left : a.chunk) * (float)a.Cg, f = nc / (n + nc), d = p.x - m;
+            m = fmaf(d, f, m);
+            q += fmaf(d, d * f * n, p.y);
+            n += nc;
+        }
+    for (int h = kl >> 1; h > 0; h >>= 1) {
+        if (k0 >= h && k0 < 2 * h) { lds[t][0] = n; lds[t][1] = m; lds[t][2] = q; }
+        __syncthreads();
+        if (k0 < h) {
+            const float* o = lds[t + h * tg];
+            if (o[0] > 0.f) {
+                const float f = o[0] / (n + o[0]), d = o[1] - m;
+                m = fmaf(d, f, m);
+                q += fmaf(d, d * f * n, o[2]);
+                n += o[0];
+            }
+        }
+        __syncthreads();
+    }
+    if (k0 == 0 && g < a.G) st[g] = make_float2(m, 1.f / sqrtf(fmaf(q, 1.f / n, a.eps)));
+    __syncthreads();
+}
+
+// the thread's channels: mean, rstd of their groups (stats: of the image), weight and bias
 template <int VEC> struct Affine {
     float mean[VEC], rstd[VEC], w[VEC], b[VEC];
-    __device__ __forceinline__ Affine(const GnArgs& a, long img, int c) {
+    __device__ __forceinline__ Affine(const GnArgs& a, const float* stats, int c) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float* s = a.stats + 2 * (img * a.G + (c + i) / a.Cg);
+            const float* s = stats + 2 * ((c + i) / a.Cg);
             mean[i] = s[0];
             rstd[i] = s[1];
             w[i] = a.w ? a.w[c + i] : 1.f;
@@ -244,23 +229,37 @@ template <int VEC> struct Affine {
 };
 
 // ------------------------------------------------------------------------------------------------ y = act(w xhat + b)
-template <class T, int VEC, int ACT>
+template <class T, int VEC, int ACT, bool PAST>
 __global__ void __launch_bounds__(THREADS) gn_apply_kernel(GnArgs a) {
     constexpr int R = in_flight<T, VEC>();
     typedef Vec<T, VEC> V;
-    const Place<VEC> w(a, blockIdx.x);
+    __shared__ float2 st[THREADS];
+    __shared__ float lds[THREADS][3];
+    // the chunks that were read last are the likeliest to be in the caches still
+    const Place<VEC> w(a, (long)gridDim.x - 1 - blockIdx.x);
+    const float* stats = a.stats + 2 * w.b * a.G;
+    if (a.join) {
+        join_stats(a, w.b, st, lds);
+        stats = reinterpret_cast<const float*>(st);
+        if (w.chunk == 0 && (int)threadIdx.x < a.G) reinterpret_cast<float2*>(a.stats)[w.b * a.G + threadIdx.x] = st[threadIdx.x];
+    }
     if (!w.active) return;
     const int c = w.c0 + w.tv * VEC;
-    Affine<VEC> k(a, w.b, c);
+    Affine<VEC> k(a, stats, c);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) k.w[i] *= k.rstd[i];
     const T* src = reinterpret_cast<const T*>(a.x) + w.b * a.xs_b + c;
     T* dst = reinterpret_cast<T*>(a.out) + w.b * a.S * a.C + c;
+    typename V::Raw next[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) next[r] = ld<V>(src + w.pixel(w.p0 + w.pl, r, a.PL) * a.xs_p);
     for (long base = w.p0 + w.pl; base < w.p1; base += (long)R * a.PL) {
         typename V::Raw raw[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            raw[r] = *reinterpret_cast<const typename V::Raw*>(src + w.pixel(base, r, a.PL) * a.xs_p);
+        for (int r = 0; r < R; ++r) {
+            raw[r] = next[r];
+            next[r] = ld<V>(src + w.pixel(base + (long)R * a.PL, r, a.PL) * a.xs_p);
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (base + (long)r * a.PL < w.p1) {
@@ -268,7 +267,7 @@ __global__ void __launch_bounds__(THREADS) gn_apply_kernel(GnArgs a) {
                 V::unpack(raw[r], v);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) v[i] = act_of<ACT>(fmaf(v[i] - k.mean[i], k.w[i], k.b[i]));
-                *reinterpret_cast<typename V::Raw*>(dst + (base + (long)r * a.PL) * a.C) = V::pack(v);
+                put<V, PAST>(dst + (base + (long)r * a.PL) * a.C, V::pack(v));
             }
     }
 }
@@ -286,7 +285,7 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_reduce_kernel(GnArgs a) {
     for (int i = 0; i < VEC; ++i) d1[i] = d2[i] = 0.f;
     const int c = w.c0 + w.tv * VEC;
     if (w.active) {
-        const Affine<VEC> k(a, w.b, c);
+        const Affine<VEC> k(a, a.stats + 2 * w.b * a.G, c);
         const T* src = reinterpret_cast<const T*>(a.x) + w.b * a.xs_b + c;
         const T* gsrc = reinterpret_cast<const T*>(a.dy) + w.b * a.ds_b + c;
         for (long base = w.p0 + w.pl; base < w.p1; base += (long)R * a.PL) {
@@ -347,6 +346,7 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_join_kernel(GnArgs a, int TC) 
         const int c = g * a.Cg + cc + tc;
         float v1 = 0.f, v2 = 0.f;
         if (ok)
+    #pragma unroll 4
             for (long k = tk; k < a.nchunk; k += NK) {
                 const float* p = a.part + 2 * (b * a.nchunk + k) * a.C + c;
                 v1 += p[0];
@@ -383,41 +383,99 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_join_kernel(GnArgs a, int TC) 
     }
 }
 
-// dw, db: chsum over the images; 16 channels x 16 image lanes per workgroup
-__global__ void __launch_bounds__(THREADS) gn_bwd_params_kernel(GnArgs a) {
-    __shared__ float s1[THREADS], s2[THREADS];
-    const int t = threadIdx.x, c = blockIdx.x * 16 + (t & 15), tb = t >> 4;
+// dw, db: [rows][2][C] sums (images, or their chunks) over the rows; 2^k >= C channels (at most 64) per workgroup, the other
+// lanes along the rows
+__device__ __forceinline__ void sum_params(const GnArgs& a, const float* rows, long n, int wg, float (*lds)[2]) {
+    int tc = 1;
+    while (tc < a.C && tc < 64) tc *= 2;
+    const int t = threadIdx.x, c = wg * tc + (t & (tc - 1)), k0 = t / tc, kl = THREADS / tc;
     float v1 = 0.f, v2 = 0.f;
     if (c < a.C)
-        for (long b = tb; b < a.B; b += 16) {
-            v1 += a.chsum[2 * b * a.C + c];
-            v2 += a.chsum[(2 * b + 1) * a.C + c];
+#pragma unroll 4
+        for (long k = k0; k < n; k += kl) {
+            v1 += rows[2 * k * a.C + c];
+            v2 += rows[(2 * k + 1) * a.C + c];
         }
-    s1[t] = v1;
-    s2[t] = v2;
+    lds[t][0] = v1;
+    lds[t][1] = v2;
     __syncthreads();
-    for (int h = 8; h > 0; h >>= 1) {
-        if (tb < h) { s1[t] += s1[t + 16 * h]; s2[t] += s2[t + 16 * h]; }
+    for (int h = kl >> 1; h > 0; h >>= 1) {
+        if (k0 < h) { lds[t][0] += lds[t + h * tc][0]; lds[t][1] += lds[t + h * tc][1]; }
         __syncthreads();
     }
-    if (tb == 0 && c < a.C) {
-        if (a.db) a.db[c] = s1[t];
-        if (a.dw) a.dw[c] = s2[t];
+    if (k0 == 0 && c < a.C) {
+        if (a.db) a.db[c] = lds[t][0];
+        if (a.dw) a.dw[c] = lds[t][1];
     }
 }
+int params_wgs(int C) {
+    int tc = 1;
+    while (tc < C && tc < 64) tc *= 2;
+    return (C + tc - 1) / tc;
+}
 
-template <class T, int VEC, int ACT>
+__global__ void __launch_bounds__(THREADS) gn_bwd_params_kernel(GnArgs a) {
+    __shared__ float lds[THREADS][2];
+    sum_params(a, a.chsum, a.B, (int)blockIdx.x, lds);
+}
+
+// gn_bwd_join_kernel's coefficients inside the pass that uses them, where an image has few chunks and channels (C <= 256, one
+// block): st[g] = mean(w dz), mean(w dz xhat)
+__device__ __forceinline__ void join_coef(const GnArgs& a, long b, float2* st, float (*lds)[2]) {
+    int tc = 1;
+    while (tc < a.C) tc *= 2;
+    const int t = threadIdx.x, c = t & (tc - 1), k0 = t / tc, kl = THREADS / tc;
+    float v1 = 0.f, v2 = 0.f;
+    if (c < a.C)
+#pragma unroll 4
+        for (int k = k0; k < (int)a.nchunk; k += kl) {
+            const float* p = a.part + 2 * (b * a.nchunk + k) * a.C + c;
+            v1 += p[0];
+            v2 += p[a.C];
+        }
+    const float w = c < a.C && a.w ? a.w[c] : 1.f;
+    lds[t][0] = v1 * w;
+    lds[t][1] = v2 * w;
+    __syncthreads();
+    for (int h = kl >> 1; h > 0; h >>= 1) {
+        if (k0 < h) { lds[t][0] += lds[t + h * tc][0]; lds[t][1] += lds[t + h * tc][1]; }
+        __syncthreads();
+    }
+    if (t < a.G) {
+        float s1 = 0.f, s2 = 0.f;
+        for (int i = 0; i < a.Cg; ++i) { s1 += lds[t * a.Cg + i][0]; s2 += lds[t * a.Cg + i][1]; }
+        const float rn = 1.f / ((float)a.S * (float)a.Cg);
+        st[t] = make_float2(s1 * rn, s2 * rn);
+    }
+    __syncthreads();
+}
+
+// dx; the last workgroups (with a.dw or a.db) sum the parameters' gradients
+template <class T, int VEC, int ACT, bool PAST>
 __global__ void __launch_bounds__(THREADS) gn_bwd_dx_kernel(GnArgs a) {
     constexpr int R = in_flight<T, VEC>() / 2;
     typedef Vec<T, VEC> V;
-    const Place<VEC> w(a, blockIdx.x);
+    __shared__ float2 st[THREADS];
+    __shared__ float lds[THREADS][2];
+    const long work = a.out ? a.B * a.nblk * a.nchunk : 0;
+    if ((long)blockIdx.x >= work) {
+        if (a.join) sum_params(a, a.part, a.B * a.nchunk, (int)(blockIdx.x - work), lds);
+        else sum_params(a, a.chsum, a.B, (int)(blockIdx.x - work), lds);
+        return;
+    }
+    const Place<VEC> w(a, work - 1 - blockIdx.x);
+    const float* coef = a.coef + 2 * w.b * a.G;
+    if (a.join) {
+        join_coef(a, w.b, st, lds);
+        coef = reinterpret_cast<const float*>(st);
+    }
     if (!w.active) return;
     const int c = w.c0 + w.tv * VEC;
-    const Affine<VEC> k(a, w.b, c);
+    const Affine<VEC> k(a, a.stats + 2 * w.b * a.G, c);
     float q1[VEC], q2[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-        const float* s = a.coef + 2 * (w.b * a.G + (c + i) / a.Cg);
+        const float* s = coef + 2 * ((c + i) / a.Cg);
         q1[i] = s[0];
         q2[i] = s[1];
     }
@@ -428,8 +486,8 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_dx_kernel(GnArgs a) {
         typename V::Raw raw[R], graw[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            raw[r] = *reinterpret_cast<const typename V::Raw*>(src + w.pixel(base, r, a.PL) * a.xs_p);
-            graw[r] = *reinterpret_cast<const typename V::Raw*>(gsrc + w.pixel(base, r, a.PL) * a.ds_p);
+            raw[r] = ld<V>(src + w.pixel(base, r, a.PL) * a.xs_p);
+            graw[r] = ld<V>(gsrc + w.pixel(base, r, a.PL) * a.ds_p);
         }
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -443,7 +501,7 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_dx_kernel(GnArgs a) {
                     const float dz = g[i] * act_slope<ACT>(fmaf(xh, k.w[i], k.b[i]));
                     v[i] = k.rstd[i] * (fmaf(dz, k.w[i], -q1[i]) - xh * q2[i]);
                 }
-                *reinterpret_cast<typename V::Raw*>(dst + (base + (long)r * a.PL) * a.C) = V::pack(v);
+                put<V, PAST>(dst + (base + (long)r * a.PL) * a.C, V::pack(v));
             }
     }
 }
@@ -451,6 +509,7 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_dx_kernel(GnArgs a) {
 // ------------------------------------------------------------------------------------------------ host
 // Number of workgroups that the chunks of a pass aim at: eight 256-thread workgroups on each of 256 CUs
 constexpr long AIM_WGS = 2048;
+constexpr int64_t PAST_BYTES = 64 << 20;            // results of a quarter of the last-level cache or more are written past it
 
 // Split of [B, S, C] for a vector of `vec` channels, `inflight` pixels a thread holds at once
 void split(GnArgs& a, int vec, int inflight) {
@@ -487,9 +546,9 @@ long max_parts(long B, long S, int C, int G, bool backward) {
 
 bool aligned(const void* p, long bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
 
-// widest vector (8, 2, 1 bf16 or 4, 1 fp32) that divides the channels, the strides and every address
+// widest vector that divides the channels, the strides and every address
 int vec_of(const GnArgs& a, int esize, bool backward) {
-    for (int vec = 16 / esize; vec > 1; vec = (esize == 2 && vec == 8) ? 2 : 1) {
+    for (int vec = 16 / esize; vec > 1; vec /= 2) {
         const long bytes = (long)vec * esize;
         bool ok = a.C % vec == 0 && a.xs_b % vec == 0 && a.xs_p % vec == 0 && aligned(a.x, bytes) && aligned(a.out, bytes);
         if (backward) ok = ok && a.ds_b % vec == 0 && a.ds_p % vec == 0 && aligned(a.dy, bytes);
@@ -498,19 +557,35 @@ int vec_of(const GnArgs& a, int esize, bool backward) {
     return 1;
 }
 
+template <class T, int VEC> void stats(const GnArgs& a, dim3 grid, hipStream_t st) {
+    const dim3 block(THREADS);
+    if (a.Cg % VEC == 0) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, 1>), grid, block, 0, st, a);
+    else if (VEC > 2 && VEC % a.Cg == 0 && VEC / a.Cg == 2) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, (VEC > 2 ? 2 : 1)>), grid, block, 0, st, a);
+    else if (VEC > 4 && VEC % a.Cg == 0 && VEC / a.Cg == 4) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, (VEC > 4 ? 4 : 1)>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gn_stats_kernel<T, VEC, VEC>), grid, block, 0, st, a);
+}
+
+template <class T, int VEC, int ACT> void apply(const GnArgs& a, dim3 grid, hipStream_t st) {
+    if (a.past) hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT, true>), grid, dim3(THREADS), 0, st, a);
+    else hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT, false>), grid, dim3(THREADS), 0, st, a);
+}
+
 template <class T, int VEC> int run_fwd(GnArgs& a, int act, hipStream_t st) {
     split(a, VEC, in_flight<T, VEC>());
     const dim3 grid((unsigned)(a.B * a.nblk * a.nchunk)), block(THREADS);
-    if (a.Cg % VEC == 0) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((gn_stats_kernel<T, VEC, false>), grid, block, 0, st, a);
+    // the statistics are joined by every workgroup that uses them where that is at most 128 values for a lane pair to read
+    a.join = a.nblk == 1 && a.G <= THREADS && a.nchunk * a.G <= 4096;
+    stats<T, VEC>(a, grid, st);
     KSR_LAUNCH_CHECK("group_norm_fwd");
-    hipLaunchKernelGGL(gn_stats_join_kernel, dim3((unsigned)((a.B * a.G + 3) / 4)), block, 0, st, a);
-    KSR_LAUNCH_CHECK("group_norm_fwd");
+    if (!a.join) {
+        hipLaunchKernelGGL(gn_stats_join_kernel, dim3((unsigned)((a.B * a.G + 3) / 4)), block, 0, st, a);
+        KSR_LAUNCH_CHECK("group_norm_fwd");
+    }
     switch (act) {
-        case KSR_ACT_NONE: hipLaunchKernelGGL((gn_apply_kernel<T, VEC, KSR_ACT_NONE>), grid, block, 0, st, a); break;
-        case KSR_ACT_RELU: hipLaunchKernelGGL((gn_apply_kernel<T, VEC, KSR_ACT_RELU>), grid, block, 0, st, a); break;
-        case KSR_ACT_SILU: hipLaunchKernelGGL((gn_apply_kernel<T, VEC, KSR_ACT_SILU>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((gn_apply_kernel<T, VEC, KSR_ACT_GELU>), grid, block, 0, st, a); break;
+        case KSR_ACT_NONE: apply<T, VEC, KSR_ACT_NONE>(a, grid, st); break;
+        case KSR_ACT_RELU: apply<T, VEC, KSR_ACT_RELU>(a, grid, st); break;
+        case KSR_ACT_SILU: apply<T, VEC, KSR_ACT_SILU>(a, grid, st); break;
+        default: apply<T, VEC, KSR_ACT_GELU>(a, grid, st); break;
     }
     KSR_LAUNCH_CHECK("group_norm_fwd");
     return KSR_OK;
@@ -518,19 +593,21 @@ template <class T, int VEC> int run_fwd(GnArgs& a, int act, hipStream_t st) {
 
 template <class T, int VEC, int ACT> int run_bwd_act(GnArgs& a, hipStream_t st) {
     split(a, VEC, in_flight<T, VEC>() / 2);
-    const dim3 grid((unsigned)(a.B * a.nblk * a.nchunk)), block(THREADS);
-    hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, VEC, ACT>), grid, block, 0, st, a);
+    const dim3 block(THREADS);
+    const long work = a.B * a.nblk * a.nchunk;
+    a.join = a.nblk == 1 && a.C <= THREADS && a.nchunk * a.C <= 4096;
+    hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, VEC, ACT>), dim3((unsigned)work), block, 0, st, a);
     KSR_LAUNCH_CHECK("group_norm_bwd");
-    int tc = 1;
-    while (tc < a.Cg && tc < 64) tc *= 2;
-    hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * a.G)), block, 0, st, a, tc);
-    KSR_LAUNCH_CHECK("group_norm_bwd");
-    if (a.dw || a.db) {
-        hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)((a.C + 15) / 16)), block, 0, st, a);
+    if (!a.join) {
+        int tc = 1;
+        while (tc < a.Cg && tc < 64) tc *= 2;
+        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * a.G)), block, 0, st, a, tc);
         KSR_LAUNCH_CHECK("group_norm_bwd");
     }
-    if (a.out) {
-        hipLaunchKernelGGL((gn_bwd_dx_kernel<T, VEC, ACT>), grid, block, 0, st, a);
+    const long wgs = (a.out ? work : 0) + (a.dw || a.db ? params_wgs(a.C) : 0);
+    if (wgs) {
+        if (a.past) hipLaunchKernelGGL((gn_bwd_dx_kernel<T, VEC, ACT, true>), dim3((unsigned)wgs), block, 0, st, a);
+        else hipLaunchKernelGGL((gn_bwd_dx_kernel<T, VEC, ACT, false>), dim3((unsigned)wgs), block, 0, st, a);
         KSR_LAUNCH_CHECK("group_norm_bwd");
     }
     return KSR_OK;
@@ -574,9 +651,13 @@ extern "C" int ksr_group_norm_fwd(const void* x, int64_t x_image_stride, int64_t
     a.x = x; a.out = y; a.w = weight; a.b = bias; a.stats = stats; a.part = ws;
     a.xs_b = x_image_stride; a.xs_p = x_pixel_stride;
     a.B = B; a.S = S; a.C = C; a.G = G; a.Cg = C / G; a.eps = eps;
-    const int vec = vec_of(a, bf16 ? 2 : 4, false);
-    if (bf16) return vec == 8 ? run_fwd<__bf16, 8>(a, act, stream) : vec == 2 ? run_fwd<__bf16, 2>(a, act, stream) : run_fwd<__bf16, 1>(a, act, stream);
-    return vec == 4 ? run_fwd<float, 4>(a, act, stream) : run_fwd<float, 1>(a, act, stream);
+    a.past = B * S * C * (bf16 ? 2 : 4) >= PAST_BYTES;
+    int vec, ne;
+    if (ksr_gn_one_fits(a, bf16 ? 2 : 4, false, vec, ne)) return ksr_gn_one_fwd(a, act, bf16 != 0, vec, ne, stream);
+    vec = vec_of(a, bf16 ? 2 : 4, false);
+    if (bf16)
+        return vec == 8 ? run_fwd<__bf16, 8>(a, act, stream) : vec == 4 ? run_fwd<__bf16, 4>(a, act, stream) : vec == 2 ? run_fwd<__bf16, 2>(a, act, stream) : run_fwd<__bf16, 1>(a, act, stream);
+    return vec == 4 ? run_fwd<float, 4>(a, act, stream) : vec == 2 ? run_fwd<float, 2>(a, act, stream) : run_fwd<float, 1>(a, act, stream);
 }
 
 extern "C" int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t x_pixel_stride, const void* dy, int64_t dy_image_stride,
@@ -589,10 +670,11 @@ extern "C" int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t
     a.x = x; a.dy = dy; a.out = dx; a.w = weight; a.b = bias; a.stats = const_cast<float*>(stats); a.dw = dweight; a.db = dbias;
     a.xs_b = x_image_stride; a.xs_p = x_pixel_stride; a.ds_b = dy_image_stride; a.ds_p = dy_pixel_stride;
     a.B = B; a.S = S; a.C = C; a.G = G; a.Cg = C / G;
+    a.past = B * S * C * (bf16 ? 2 : 4) >= PAST_BYTES;
     if (B == 0 || S == 0) {                               // empty sums
         a.B = 0;
         if (!dweight && !dbias) return KSR_OK;
-        hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)((C + 15) / 16)), dim3(THREADS), 0, stream, a);
+        hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)params_wgs(C)), dim3(THREADS), 0, stream, a);
         KSR_LAUNCH_CHECK("group_norm_bwd");
         return KSR_OK;
     }
@@ -602,7 +684,18 @@ extern "C" int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t
     a.coef = ws;
     a.chsum = a.coef + 2 * B * G;
     a.part = a.chsum + 2 * B * C;
-    const int vec = vec_of(a, bf16 ? 2 : 4, true);
-    if (bf16) return vec == 8 ? run_bwd<__bf16, 8>(a, act, stream) : vec == 2 ? run_bwd<__bf16, 2>(a, act, stream) : run_bwd<__bf16, 1>(a, act, stream);
-    return vec == 4 ? run_bwd<float, 4>(a, act, stream) : run_bwd<float, 1>(a, act, stream);
+    int vec, ne;
+    if (ksr_gn_one_fits(a, bf16 ? 2 : 4, true, vec, ne)) {
+        if (!dweight && !dbias) a.chsum = nullptr;
+        if (int rc = ksr_gn_one_bwd(a, act, bf16 != 0, vec, ne, stream)) return rc;
+        if (B > 1 && a.chsum) {
+            hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)params_wgs(C)), dim3(THREADS), 0, stream, a);
+            KSR_LAUNCH_CHECK("group_norm_bwd");
+        }
+        return KSR_OK;
+    }
+    vec = vec_of(a, bf16 ? 2 : 4, true);
+    if (bf16)
+        return vec == 8 ? run_bwd<__bf16, 8>(a, act, stream) : vec == 4 ? run_bwd<__bf16, 4>(a, act, stream) : vec == 2 ? run_bwd<__bf16, 2>(a, act, stream) : run_bwd<__bf16, 1>(a, act, stream);
+    return vec == 4 ? run_bwd<float, 4>(a, act, stream) : vec == 2 ? run_bwd<float, 2>(a, act, stream) : run_bwd<float, 1>(a, act, stream);
 }

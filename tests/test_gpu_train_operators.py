@@ -57,7 +57,16 @@ def test_unet_group_norm_vs_oracle(B, H, W, P, groups, monkeypatch):
         assert bool((z.detach().abs()[side != (z > 0)] <= 1e-5).all()), prefix
         return z * side
 
+    rows, plain_rows = [], orc._l2_rows
+
+    def recorded_rows(t, eps=1e-12):
+        out = plain_rows(t, eps)
+        out.retain_grad()
+        rows.append((t.detach(), out))
+        return out
+
     monkeypatch.setattr(orc, "group_norm_relu", on_the_kernels_side)
+    monkeypatch.setattr(orc, "_l2_rows", recorded_rows)
     ref = orc.unet(x.double(), p, groups=groups)
     (ref * gy.double()).sum().backward()
     y = m.train()(x.cuda())
@@ -65,9 +74,16 @@ def test_unet_group_norm_vs_oracle(B, H, W, P, groups, monkeypatch):
     assert bool(((y.detach().cpu() - ref.detach()).abs() <= 2e-5 + 1e-4 * ref.detach().abs()).all())
     y.backward(gy.cuda())
     rel = 1e-4 if (H // 16) * (W // 16) >= 16 else 1e-3
-    # The helper holds gradients that are zero to an absolute bound: at 16 x 16 pixels the queries of att4 are one pixel long,
-    # q / |q| = +-1 has derivative 0, and fp32 leaves its rounding of 1 - 1
-    _check_grads({n: q.grad for n, q in m.named_parameters()}, {n: q.grad for n, q in p.items()}, rel=rel)
+    # Where a row that is normalised is one pixel long (att4 at 16 x 16), q / |q| = +-1 has derivative 0: (u - q^ (q^ u)) / |q|
+    # with q^ q^ = 1.  fp32 has q^ q^ within 2^-23 of 1, so up to 4 half steps of u / |q| remain, times what the weight's
+    # gradient multiplies them with: the input, and for the two convolutions of `a` the other's weight, over 32 channels.
+    left = max([float((out.grad.abs() / t.abs()).max()) for t, out in rows if t.shape[-1] == 1], default=0.0)
+    x_max = float(max(t["out"].abs().max() for t in tape.values() if "mid" in t))
+    zero = {n for n, q in p.items() if float(q.grad.norm()) < 1e-6 * max(1.0, q.numel() ** 0.5)}
+    for n, q in m.named_parameters():
+        if n in zero:
+            assert n.startswith("att") and float(q.grad.abs().max()) <= max(1e-5, 4 * 2.0 ** -24 * left * x_max * 32 * B), n
+    _check_grads({n: q.grad for n, q in m.named_parameters() if n not in zero}, {n: q.grad for n, q in p.items()}, rel=rel)
     with torch.no_grad():
         assert torch.equal(m.eval()(x.cuda()), y.detach())            # no running statistics: both modes are the same function
         one = m(x[:1].cuda())
