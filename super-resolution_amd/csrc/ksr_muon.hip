@@ -414,7 +414,7 @@ struct LMat {
     int m, n, mp, np, tall;
     int sub0, nsub;                 // matrices sub0 .. sub0 + nsub - 1 of the entry's batch
     int parts;
-    int first, sym, full;           // matrices, tiles of the lower triangles, tiles of X in the entries before this one
+    int first, sym, full[2];        // matrices, tiles of the lower triangles, of X and of the result in the entries before this one
 };
 struct Large {
     char* ws;
@@ -581,12 +581,19 @@ __host__ __device__ inline int chunk_of(int k) {
     return c;
 }
 
-template <int TILE, bool SPLIT, int KIND>
+// tiles of a product: of the lower triangle, or of X (U, transposed or not) with the last row of tiles possibly cut off
+template <int TM, int TN, int KIND> __host__ __device__ inline int tiles_of(const LMat& e) {
+    if (KIND == A_OF_X || KIND == B_OF_A) return e.mp / TM * (e.mp / TM + 1) / 2;
+    const bool swap = KIND == X_LAST && e.tall;
+    return ((swap ? e.np : e.mp) + TM - 1) / TM * ((swap ? e.mp : e.np) / TN);
+}
+
+template <int TM, int TN, int BK, int NST, bool SPLIT, int KIND>
 __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
-    constexpr int BK = SPLIT ? 32 : 64, NP = SPLIT ? 2 : 1, W = TILE / 2, NT = W / 32, CH = BK / 8, NST = TILE == 64 ? 4 : 2;
-    constexpr int OPBYTES = TILE * BK * 2, STAGE = 2 * NP * OPBYTES;
-    constexpr int STG = TILE + 8;                                       // halves per row of the output tile in LDS
-    static_assert(NST * STAGE >= TILE * STG * 2, "the output tile reuses the stages");
+    constexpr int NP = SPLIT ? 2 : 1, WM = TM / 2, WN = TN / 2, MT = WM / 32, NT = WN / 32, CH = BK / 8;
+    constexpr int PBYTES = TM * BK * 2, QBYTES = TN * BK * 2, STAGE = NP * (PBYTES + QBYTES);
+    static_assert(NST * STAGE >= TM * (TN + 8) * 2 && NST * STAGE >= TN * (TM + 8) * 2, "the output tile reuses the stages");
+    static_assert((KIND != A_OF_X && KIND != B_OF_A) || TM == TN, "the triangle's tiles are square");
     __shared__ __attribute__((aligned(16))) char lds[NST * STAGE];
     __shared__ int arrived;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1;
@@ -594,13 +601,13 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
     int t, slice = 0, slices = 1, slot = 0, q = 0;      // slot: of the tile's first partial sums
     if ((int)blockIdx.x < a.whole) {
         t = (int)ksr_xcd_contiguous(blockIdx.x, (unsigned)a.whole);
-        while (q + 1 < a.l.count && t >= (SYM ? a.l.e[q + 1].sym : a.l.e[q + 1].full)) ++q;
+        while (q + 1 < a.l.count && t >= (SYM ? a.l.e[q + 1].sym : a.l.e[q + 1].full[KIND == X_LAST])) ++q;
     } else {
         // entries whose tiles are cut: each with its own number of chunks
         int rest = (int)blockIdx.x - a.whole;
         for (;; ++q) {
             const LMat& e = a.l.e[q];
-            const int first = SYM ? e.sym : e.full, mt = e.mp / TILE, tiles = e.nsub * (SYM ? mt * (mt + 1) / 2 : mt * (e.np / TILE));
+            const int first = SYM ? e.sym : e.full[KIND == X_LAST], tiles = e.nsub * tiles_of<TM, TN, KIND>(e);
             const int from = a.whole > first ? a.whole : first, cut = first + tiles - from;       // tiles of this entry in the rest
             if (cut <= 0) continue;
             const int ch = chunk_of(KIND == A_OF_X ? e.n : e.m), kp = KIND == A_OF_X ? e.np : e.mp, n = a.cut ? (kp + ch - 1) / ch : 1;
@@ -615,21 +622,20 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
         }
     }
     const LMat& l = a.l.e[q];
-    t -= SYM ? l.sym : l.full;
-    const int mt = l.mp / TILE, nt = l.np / TILE, per = SYM ? mt * (mt + 1) / 2 : mt * nt;
+    t -= SYM ? l.sym : l.full[KIND == X_LAST];
+    const bool swap = KIND == X_LAST && l.tall;
+    const int mt = (swap ? l.np + TM - 1 : l.mp + TM - 1) / TM, nt = (swap ? l.mp : l.np) / TN, per = SYM ? mt * (mt + 1) / 2 : mt * nt;
     const int at = t / per, sub = l.sub0 + at;
     t -= at * per;
     const Offsets of(l.mp, l.np, SPLIT);
     char* ws = a.l.ws + l.off + at * of.per;
-    const bool swap = KIND == X_LAST && l.tall;
     int ti, tj;
     if constexpr (SYM) {
         ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
         while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
         while (ti * (ti + 1) / 2 > t) --ti;
         tj = t - ti * (ti + 1) / 2;
-    } else if (swap) { ti = t / mt; tj = t % mt; }
-    else { ti = t % mt; tj = t / mt; }
+    } else { ti = t % mt; tj = t / mt; }
     const _Float16* R = reinterpret_cast<const _Float16*>(ws + of.r);
     const _Float16* xt = reinterpret_cast<const _Float16*>(ws + of.xt(a.k));
     const _Float16 *P, *Q;
@@ -643,43 +649,50 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
         pp = swap ? (long)l.np * l.mp : (long)l.mp * l.mp;
         qp = swap ? (long)l.mp * l.mp : (long)l.np * l.mp;
     }
-    P += (long)ti * TILE * K;
-    Q += (long)tj * TILE * K;
+    P += (long)ti * TM * K;
+    Q += (long)tj * TN * K;
+    const int rows = SYM ? TM : (swap ? l.np : l.mp) - ti * TM;        // of P; fewer than TM in the last tile of an odd number of 128s
     // LDS-DMA: one instruction of a wave brings 64 chunks of 16 bytes; lane -> (row, slot), the chunk that belongs there
-    constexpr int ROWS = 64 / CH, NI = TILE / ROWS / 4;                 // rows per instruction, instructions per wave and operand plane
-    constexpr int PER_STAGE = 2 * NP * NI;                              // a wave's instructions per stage
+    constexpr int ROWS = 64 / CH, PI = TM / ROWS / 4, QI = TN / ROWS / 4;        // rows per instruction, instructions per wave and plane
+    constexpr int PER_STAGE = NP * (PI + QI);                           // a wave's instructions per stage
     const int drow = lane / CH, dslot = lane % CH;
     auto f = [](int row) { return CH == 8 ? (row & 7) : ((row >> 1) & 3); };
     auto fill = [&](int kt) {
-        const int st = kt % NST;
+        char* to = lds + kt % NST * STAGE;
 #pragma unroll
-        for (int op = 0; op < 2; ++op)
+        for (int pl = 0; pl < NP; ++pl) {
 #pragma unroll
-            for (int pl = 0; pl < NP; ++pl)
+            for (int i = 0; i < PI; ++i) {
+                const int row = (wave * PI + i) * ROWS + drow;
+                const _Float16* src = P + pl * pp + (long)(TM == TN || row < rows ? row : 0) * K + kt * BK + 8 * (dslot ^ f(row));
+                ksr_dma16<false>(src, to + pl * PBYTES + (wave * PI + i) * 1024);
+            }
 #pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const int row = (wave * NI + i) * ROWS + drow;
-                    const _Float16* src = (op ? Q + pl * qp : P + pl * pp) + (long)row * K + kt * BK + 8 * (dslot ^ f(row));
-                    ksr_dma16<false>(src, lds + st * STAGE + (op * NP + pl) * OPBYTES + (wave * NI + i) * 1024);
-                }
+            for (int i = 0; i < QI; ++i) {
+                const int row = (wave * QI + i) * ROWS + drow;
+                const _Float16* src = Q + pl * qp + (long)row * K + kt * BK + 8 * (dslot ^ f(row));
+                ksr_dma16<false>(src, to + NP * PBYTES + pl * QBYTES + (wave * QI + i) * 1024);
+            }
+        }
     };
-    auto frag = [&](int st, int op, int pl, int row, int ks) {
+    auto frag = [&](int st, int at_byte, int row, int ks) {
         const int chunk = (2 * ks + (lane >> 5)) ^ f(row);
-        return *reinterpret_cast<const h8*>(lds + st * STAGE + (op * NP + pl) * OPBYTES + row * (BK * 2) + 16 * chunk);
+        return *reinterpret_cast<const h8*>(lds + st * STAGE + at_byte + row * (BK * 2) + 16 * chunk);
     };
     // hi lo + lo hi have accumulators of their own: added to the large sum one by one they would round it three times a step
-    f32x16 acc[NT][NT] = {}, low[SPLIT ? NT : 1][SPLIT ? NT : 1] = {}, sum[NT][NT] = {};
+    f32x16 acc[MT][NT] = {}, low[SPLIT ? MT : 1][SPLIT ? NT : 1] = {}, sum[SPLIT ? MT : 1][SPLIT ? NT : 1] = {};
     const int chunk = chunk_of(KIND == A_OF_X ? l.n : l.m) / BK, nk = K / BK;
     const int k0 = slices > 1 ? slice * chunk : 0, k1 = slices > 1 && k0 + chunk < nk ? k0 + chunk : nk;
     auto flush = [&]() {
+        if constexpr (SPLIT)
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+            for (int x = 0; x < MT; ++x)
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                if constexpr (SPLIT) { acc[x][y] += low[x][y]; low[x][y] = f32x16{}; }
-                sum[x][y] += acc[x][y];
-                acc[x][y] = f32x16{};
-            }
+                for (int y = 0; y < NT; ++y) {
+                    acc[x][y] += low[x][y];
+                    sum[x][y] += acc[x][y];
+                    acc[x][y] = low[x][y] = f32x16{};
+                }
     };
     for (int kt = k0; kt < k0 + NST - 1 && kt < k1; ++kt) fill(kt);
     for (int kt = k0; kt < k1; ++kt) {
@@ -691,18 +704,19 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
         const int st = kt % NST;
 #pragma unroll
         for (int ks = 0; ks < BK / 16; ++ks) {
-            h8 ph[NT], qh[NT], pl[NT], ql[NT];
+            h8 ph[MT], qh[NT], pl[SPLIT ? MT : 1], ql[SPLIT ? NT : 1];
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-                ph[x] = frag(st, 0, 0, wr * W + 32 * x + (lane & 31), ks);
-                qh[x] = frag(st, 1, 0, wc * W + 32 * x + (lane & 31), ks);
-                if constexpr (SPLIT) {
-                    pl[x] = frag(st, 0, 1, wr * W + 32 * x + (lane & 31), ks);
-                    ql[x] = frag(st, 1, 1, wc * W + 32 * x + (lane & 31), ks);
-                }
+            for (int x = 0; x < MT; ++x) {
+                ph[x] = frag(st, 0, wr * WM + 32 * x + (lane & 31), ks);
+                if constexpr (SPLIT) pl[x] = frag(st, PBYTES, wr * WM + 32 * x + (lane & 31), ks);
             }
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
+            for (int y = 0; y < NT; ++y) {
+                qh[y] = frag(st, NP * PBYTES, wc * WN + 32 * y + (lane & 31), ks);
+                if constexpr (SPLIT) ql[y] = frag(st, NP * PBYTES + QBYTES, wc * WN + 32 * y + (lane & 31), ks);
+            }
+#pragma unroll
+            for (int x = 0; x < MT; ++x)
 #pragma unroll
                 for (int y = 0; y < NT; ++y) {
                     acc[x][y] = mfma(ph[x], qh[y], acc[x][y]);
@@ -712,19 +726,24 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                     }
                 }
         }
-        if (((kt + 1) & (chunk - 1)) == 0 || kt + 1 == k1) flush();      // chunk is a power of two
+        if (SPLIT && (((kt + 1) & (chunk - 1)) == 0 || kt + 1 == k1)) flush();      // chunk is a power of two
     }
+    if constexpr (SPLIT)
+#pragma unroll
+        for (int x = 0; x < MT; ++x)
+#pragma unroll
+            for (int y = 0; y < NT; ++y) acc[x][y] = sum[x][y];
     if (slices > 1) {
         int* counter = reinterpret_cast<int*>(a.l.ws + a.l.o_part) + slot;
-        float* part = reinterpret_cast<float*>(a.l.ws + a.l.o_part + 4l * SLOTS) + (long)slot * TILE * TILE + threadIdx.x;
-        float* own = part + (long)slice * TILE * TILE;
+        float* part = reinterpret_cast<float*>(a.l.ws + a.l.o_part + 4l * SLOTS) + (long)slot * TM * TN + threadIdx.x;
+        float* own = part + (long)slice * TM * TN;
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int x = 0; x < MT; ++x)
 #pragma unroll
             for (int y = 0; y < NT; ++y)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    __hip_atomic_store(own + ((x * NT + y) * 16 + r) * 256, sum[x][y][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(own + ((x * NT + y) * 16 + r) * 256, acc[x][y][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         // Device-scope accesses go past the caches of the eight dies, and a wave's are complete when its count of outstanding ones
         // is 0: the sums are in place before the arrival is counted.  (A release fence would write back a whole L2 per workgroup.)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -734,17 +753,17 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
         if (arrived != slices - 1) return;
         if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);       // for the next launch
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int x = 0; x < MT; ++x)
 #pragma unroll
-            for (int y = 0; y < NT; ++y) sum[x][y] = f32x16{};
+            for (int y = 0; y < NT; ++y) acc[x][y] = f32x16{};
         for (int w = 0; w < slices; ++w)
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
+            for (int x = 0; x < MT; ++x)
 #pragma unroll
                 for (int y = 0; y < NT; ++y)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        sum[x][y][r] += __hip_atomic_load(part + (long)w * TILE * TILE + ((x * NT + y) * 16 + r) * 256, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        acc[x][y][r] += __hip_atomic_load(part + (long)w * TM * TN + ((x * NT + y) * 16 + r) * 256, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     ksr_lds_barrier();                                  // LDS is free for the output tile
     // ---- values
@@ -757,15 +776,15 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
     const Apply ap(sp, mat);
     const int mode = sp.muon ? MUON : sp.bf16 ? BF16 : F32;
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+    for (int x = 0; x < MT; ++x)
 #pragma unroll
         for (int y = 0; y < NT; ++y)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int row0 = ti * TILE + wr * W + 32 * x + 8 * g + 4 * (lane >> 5), c = tj * TILE + wc * W + 32 * y + (lane & 31);
+                const int row0 = ti * TM + wr * WM + 32 * x + 8 * g + 4 * (lane >> 5), c = tj * TN + wc * WN + 32 * y + (lane & 31);
                 float v[4];
 #pragma unroll
-                for (int z = 0; z < 4; ++z) v[z] = sum[x][y][4 * g + z];
+                for (int z = 0; z < 4; ++z) v[z] = acc[x][y][4 * g + z];
                 if constexpr (KIND == A_OF_X) {
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
@@ -786,7 +805,7 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                             v[z] = 0.f;
                         } else v[z] = S * (sp.b * r + sp.c * ((di + dc) * r + sq));
                     }
-                } else {
+                } else if (TM == TN || row0 - ti * TM < rows) {
                     const float alpha = xi * INV_S;
                     const long plane = (long)l.mp * l.np;
                     if (!swap) {                        // rows are i, columns j
@@ -818,7 +837,8 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                     }
                 }
 #pragma unroll
-                for (int z = 0; z < 4; ++z) sum[x][y][4 * g + z] = v[z];
+                for (int z = 0; z < 4; ++z) acc[x][y][4 * g + z] = v[z];
+                if (TM != TN && g == 3) __builtin_amdgcn_sched_barrier(0);        // more of X^T in flight would spill
             }
     if constexpr (KIND == X_LAST) return;
     // ---- the tile and its transpose, hi and lo, through LDS: 16-byte stores of whole rows
@@ -839,33 +859,42 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
         for (int tr = 0; tr < 2; ++tr) {
             if (tr == 1 && KIND != X_NEXT && ti == tj) continue;
             if (tr == 0 && pl == 1 && !SPLIT) continue;              // X's lo is only read through X^T (the linear term)
+            if constexpr (TM != TN)                                  // nothing rounded is kept for the next round: it would spill
 #pragma unroll
-            for (int x = 0; x < NT; ++x)
+                for (int x = 0; x < MT; ++x)
+#pragma unroll
+                    for (int y = 0; y < NT; ++y) asm volatile("" : "+v"(acc[x][y]));
+#pragma unroll
+            for (int x = 0; x < MT; ++x)
 #pragma unroll
                 for (int y = 0; y < NT; ++y)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const int r = wr * W + 32 * x + 8 * g + 4 * (lane >> 5), c = wc * W + 32 * y + (lane & 31);
+                        const int r = wr * WM + 32 * x + 8 * g + 4 * (lane >> 5), c = wc * WN + 32 * y + (lane & 31);
                         h4 w;
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            const float v = sum[x][y][4 * g + z];
+                            const float v = acc[x][y][4 * g + z];
                             const _Float16 hi = (_Float16)v;
                             w[z] = pl ? (_Float16)(v - (float)hi) : hi;
                         }
-                        if (tr) *reinterpret_cast<h4*>(stage + c * STG + r) = w;
+                        if (tr) *reinterpret_cast<h4*>(stage + c * (TM + 8) + r) = w;
                         else {
 #pragma unroll
-                            for (int z = 0; z < 4; ++z) stage[(r + z) * STG + c] = w[z];
+                            for (int z = 0; z < 4; ++z) stage[(r + z) * (TN + 8) + c] = w[z];
                         }
                     }
             __syncthreads();
             _Float16* o = (tr ? outt : out) + pl * plane;
             const long lo = tr ? ldt : ld;
-            const int r0 = (tr ? tj : ti) * TILE, c0 = (tr ? ti : tj) * TILE;
-            for (int w = threadIdx.x; w < TILE * (TILE / 8); w += 256) {
-                const int r = w / (TILE / 8), c = w % (TILE / 8) * 8;
-                *reinterpret_cast<uint4*>(o + (long)(r0 + r) * lo + c0 + c) = *reinterpret_cast<const uint4*>(stage + r * STG + c);
+            const int r0 = tr ? tj * TN : ti * TM, c0 = tr ? ti * TM : tj * TN;
+            // what lies beyond an odd number of 128s is not stored
+            const int nr = tr ? TN : rows < TM ? rows : TM, nc = tr ? (rows < TM ? rows : TM) : TN;
+            const int pitch = tr ? TM + 8 : TN + 8, per_row = (tr ? TM : TN) / 8;
+            for (int w = threadIdx.x; w < TM * TN / 8; w += 256) {
+                const int r = w / per_row, c = w % per_row * 8;
+                if (TM == TN || (r < nr && c < nc))
+                    *reinterpret_cast<uint4*>(o + (long)(r0 + r) * lo + c0 + c) = *reinterpret_cast<const uint4*>(stage + r * pitch + c);
             }
             __syncthreads();
         }
@@ -892,7 +921,7 @@ long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& s
         sub = sub0;
         long off = 0;
         int matrices = 0;
-        long sym = 0, full = 0;
+        long full = 0;
         for (; entry < count && l.count < MAX_LARGE; ++entry, sub = 0) {
             const KsrMatrix& k = mats[entry];
             if (empty(k) || is_small(k.rows, k.cols)) continue;
@@ -917,12 +946,9 @@ long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& s
             e.parts = elements / 8192 < 1 ? 1 : elements / 8192 < NORM_PARTS ? (int)(elements / 8192) : NORM_PARTS;
             e.off = off;
             e.first = matrices;
-            e.sym = (int)sym;
-            e.full = (int)full;
             m[l.count++] = Mat{k.src, k.dst, k.momentum, (long)k.row_stride, (long)k.col_stride, (long)k.batch_stride, k.rows, k.cols, k.batch, 0};
             off += e.nsub * per;
             matrices += e.nsub;
-            sym += e.nsub * (mt * (mt + 1) / 2);
             full += e.nsub * mt * nt;
             if (e.nsub < left) { sub += e.nsub; break; }
         }
@@ -963,21 +989,24 @@ template <int MODE, bool SPLIT> void start_large(const LargeArgs& a, hipStream_t
     hipLaunchKernelGGL((ns_prepare_kernel<MODE, SPLIT>), dim3(tiles, matrices), dim3(256), 0, st, a);
 }
 
-template <int TILE, bool SPLIT, int KIND> void product(LargeArgs& a, hipStream_t st) {
+template <int TM, int TN, int BK, int NST, bool SPLIT, int KIND> void product(LargeArgs& a, hipStream_t st) {
     constexpr bool SYM = KIND == A_OF_X || KIND == B_OF_A;
-    const LMat& back = a.l.e[a.l.count - 1];
-    auto tiles_of = [](const LMat& e) { return e.nsub * (SYM ? e.mp / TILE * (e.mp / TILE + 1) / 2 : e.mp / TILE * (e.np / TILE)); };
-    const int tiles = (SYM ? back.sym : back.full) + tiles_of(back);
+    int tiles = 0;
+    for (int i = 0; i < a.l.count; ++i) {
+        LMat& e = a.l.e[i];
+        (SYM ? e.sym : e.full[KIND == X_LAST]) = tiles;
+        tiles += e.nsub * tiles_of<TM, TN, KIND>(e);
+    }
     a.whole = tiles / CUS * CUS;
     long cut = 0;                                       // workgroups if every chunk of the rest has one
     for (int i = 0; i < a.l.count; ++i) {
         const LMat& e = a.l.e[i];
-        const int first = SYM ? e.sym : e.full, from = a.whole > first ? a.whole : first, n = first + tiles_of(e) - from;
+        const int first = SYM ? e.sym : e.full[KIND == X_LAST], from = a.whole > first ? a.whole : first, n = first + e.nsub * tiles_of<TM, TN, KIND>(e) - from;
         const int ch = chunk_of(KIND == A_OF_X ? e.n : e.m), kp = KIND == A_OF_X ? e.np : e.mp;
         if (n > 0) cut += (long)n * ((kp + ch - 1) / ch);
     }
-    a.cut = cut <= SLOTS;
-    hipLaunchKernelGGL((ns_gemm_kernel<TILE, SPLIT, KIND>), dim3((unsigned)(a.cut ? a.whole + cut : tiles)), dim3(256), 0, st, a);
+    a.cut = cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile;
+    hipLaunchKernelGGL((ns_gemm_kernel<TM, TN, BK, NST, SPLIT, KIND>), dim3((unsigned)(a.cut ? a.whole + cut : tiles)), dim3(256), 0, st, a);
 }
 
 template <int TILE, bool SPLIT> int run_large(LargeArgs& a, hipStream_t st) {
@@ -986,11 +1015,14 @@ template <int TILE, bool SPLIT> int run_large(LargeArgs& a, hipStream_t st) {
     else if (mode == BF16) start_large<BF16, SPLIT>(a, st);
     else start_large<MUON, SPLIT>(a, st);
     KSR_LAUNCH_CHECK("muon_batch");
+    constexpr int BK = SPLIT ? 32 : 64, NST = TILE == 64 ? 4 : 2;
+    constexpr bool WIDE = TILE == 128 && !SPLIT;       // X in 256 x 128: a wave's 128 x 64 needs 3/4 of the LDS reads per product
+    constexpr int XM = WIDE ? 256 : TILE, XK = WIDE ? 32 : BK, XS = WIDE ? 3 : NST;
     for (a.k = 0; a.k < a.s.steps; ++a.k) {
-        product<TILE, SPLIT, A_OF_X>(a, st);
-        product<TILE, SPLIT, B_OF_A>(a, st);
-        if (a.k + 1 < a.s.steps) product<TILE, SPLIT, X_NEXT>(a, st);
-        else product<TILE, SPLIT, X_LAST>(a, st);
+        product<TILE, TILE, BK, NST, SPLIT, A_OF_X>(a, st);
+        product<TILE, TILE, BK, NST, SPLIT, B_OF_A>(a, st);
+        if (a.k + 1 < a.s.steps) product<XM, TILE, XK, XS, SPLIT, X_NEXT>(a, st);
+        else product<XM, TILE, XK, XS, SPLIT, X_LAST>(a, st);
         KSR_LAUNCH_CHECK("muon_batch");
     }
     return KSR_OK;
