@@ -402,6 +402,8 @@ __global__ void __launch_bounds__(512) ns_small_kernel(Mats p) {
 // ================================================================================================ large matrices
 // All matrices of a call that are not small run together, whatever their shapes: per step one launch for A, one for B and one for
 // the next X, over the tiles of all of them.
+// Layout of every plane: blocks of 32 columns, row after row within a block, so that 16 rows of a block are 1 KB without a gap:
+// the products are bound by their loads from the L2, and rows of 64 or 128 bytes a pitch apart reach two thirds of the rate.
 // Buffers of one matrix, padded to the tile in both directions with zeros that every step reproduces (A, B and X of a zero row
 // or column are zero), so that no product needs a bounds check:  X [mp][np] and X^T [np][mp] (twice), R and B [mp][mp].  With X
 // in both orders each of the three products contracts the contiguous dimension of both operands.
@@ -422,6 +424,8 @@ struct Large {
     int count, tile, split;
     LMat e[MAX_LARGE];
 };
+
+__device__ __forceinline__ long place(int rows, int r, int k) { return ((long)(k >> 5) * rows + r) * 32 + (k & 31); }
 
 __host__ __device__ inline long align256(long v) { return (v + 255) / 256 * 256; }
 struct Offsets {
@@ -554,8 +558,9 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
 #pragma unroll
     for (int pl = 0; pl < 2; ++pl)
         for (int t = threadIdx.x; t < 4096; t += 256) {
-            if (SPLIT || pl == 0) x[pl * plane + (long)(i0 + (t >> 6)) * le.np + j0 + (t & 63)] = tile[pl][t >> 6][t & 63];
-            xt[pl * plane + (long)(j0 + (t >> 6)) * le.mp + i0 + (t & 63)] = tile[pl][t & 63][t >> 6];
+            const int r = (t >> 5) & 63, k = (t >> 11) * 32 + (t & 31);
+            if (SPLIT || pl == 0) x[pl * plane + place(le.mp, i0 + r, j0 + k)] = tile[pl][r][k];
+            xt[pl * plane + place(le.np, j0 + r, i0 + k)] = tile[pl][k][r];
         }
 }
 
@@ -640,17 +645,19 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
     const _Float16* xt = reinterpret_cast<const _Float16*>(ws + of.xt(a.k));
     const _Float16 *P, *Q;
     long pp, qp;                                        // distance of the lo plane
-    int K;
-    if constexpr (KIND == A_OF_X) { P = Q = reinterpret_cast<const _Float16*>(ws + of.x); K = l.np; pp = qp = (long)l.mp * l.np; }
-    else if constexpr (KIND == B_OF_A) { P = Q = R; K = l.mp; pp = qp = (long)l.mp * l.mp; }
+    int K, pr, qr;                                      // columns, rows of P's and Q's planes
+    if constexpr (KIND == A_OF_X) { P = Q = reinterpret_cast<const _Float16*>(ws + of.x); K = l.np; pr = qr = l.mp; pp = qp = (long)l.mp * l.np; }
+    else if constexpr (KIND == B_OF_A) { P = Q = R; K = pr = qr = l.mp; pp = qp = (long)l.mp * l.mp; }
     else {
         const _Float16* B = reinterpret_cast<const _Float16*>(ws + of.b);
         P = swap ? xt : B; Q = swap ? B : xt; K = l.mp;
-        pp = swap ? (long)l.np * l.mp : (long)l.mp * l.mp;
-        qp = swap ? (long)l.mp * l.mp : (long)l.np * l.mp;
+        pr = swap ? l.np : l.mp;
+        qr = swap ? l.mp : l.np;
+        pp = (long)pr * K;
+        qp = (long)qr * K;
     }
-    P += (long)ti * TM * K;
-    Q += (long)tj * TN * K;
+    P += (long)ti * TM * 32;
+    Q += (long)tj * TN * 32;
     const int rows = SYM ? TM : (swap ? l.np : l.mp) - ti * TM;        // of P; fewer than TM in the last tile of an odd number of 128s
     // LDS-DMA: one instruction of a wave brings 64 chunks of 16 bytes; lane -> (row, slot), the chunk that belongs there
     constexpr int ROWS = 64 / CH, PI = TM / ROWS / 4, QI = TN / ROWS / 4;        // rows per instruction, instructions per wave and plane
@@ -664,13 +671,13 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
 #pragma unroll
             for (int i = 0; i < PI; ++i) {
                 const int row = (wave * PI + i) * ROWS + drow;
-                const _Float16* src = P + pl * pp + (long)(TM == TN || row < rows ? row : 0) * K + kt * BK + 8 * (dslot ^ f(row));
+                const _Float16* src = P + pl * pp + place(pr, TM == TN || row < rows ? row : 0, kt * BK + 8 * (dslot ^ f(row)));
                 ksr_dma16<false>(src, to + pl * PBYTES + (wave * PI + i) * 1024);
             }
 #pragma unroll
             for (int i = 0; i < QI; ++i) {
                 const int row = (wave * QI + i) * ROWS + drow;
-                const _Float16* src = Q + pl * qp + (long)row * K + kt * BK + 8 * (dslot ^ f(row));
+                const _Float16* src = Q + pl * qp + place(qr, row, kt * BK + 8 * (dslot ^ f(row)));
                 ksr_dma16<false>(src, to + NP * PBYTES + pl * QBYTES + (wave * QI + i) * 1024);
             }
         }
@@ -679,54 +686,65 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
         const int chunk = (2 * ks + (lane >> 5)) ^ f(row);
         return *reinterpret_cast<const h8*>(lds + st * STAGE + at_byte + row * (BK * 2) + 16 * chunk);
     };
-    // hi lo + lo hi have accumulators of their own: added to the large sum one by one they would round it three times a step
-    f32x16 acc[MT][NT] = {}, low[SPLIT ? MT : 1][SPLIT ? NT : 1] = {}, sum[SPLIT ? MT : 1][SPLIT ? NT : 1] = {};
+    f32x16 acc[MT][NT] = {}, sum[SPLIT ? MT : 1][SPLIT ? NT : 1] = {};
     const int chunk = chunk_of(KIND == A_OF_X ? l.n : l.m) / BK, nk = K / BK;
     const int k0 = slices > 1 ? slice * chunk : 0, k1 = slices > 1 && k0 + chunk < nk ? k0 + chunk : nk;
-    auto flush = [&]() {
-        if constexpr (SPLIT)
-#pragma unroll
-            for (int x = 0; x < MT; ++x)
-#pragma unroll
-                for (int y = 0; y < NT; ++y) {
-                    acc[x][y] += low[x][y];
-                    sum[x][y] += acc[x][y];
-                    acc[x][y] = low[x][y] = f32x16{};
-                }
-    };
-    for (int kt = k0; kt < k0 + NST - 1 && kt < k1; ++kt) fill(kt);
-    for (int kt = k0; kt < k1; ++kt) {
-        // stage kt has landed (of the NST - 2 younger ones this wave's transfers may be in flight, if there are that many), and the
-        // stage that is filled next has been read by every wave
+    h8 ph[2][MT], qh[2][NT], pl[2][SPLIT ? MT : 1], ql[2][SPLIT ? NT : 1];
+    // Two sets of operands: 16 columns are multiplied while the next 16 come out of LDS, also across a stage's end, so that the
+    // barrier and the LDS' latency lie behind matrix work
+    auto stage_ready = [&](int kt) {
+        // stage kt has landed (of the NST - 2 younger ones this wave's transfers may be in flight, if there are that many), and
+        // every wave has read all of stage kt - 1, whose place the next one takes
         if (kt + NST - 2 < k1) ksr_dma_barrier_but<PER_STAGE*(NST - 2)>();
         else ksr_dma_barrier();
         if (kt + NST - 1 < k1) fill(kt + NST - 1);
+    };
+    auto load = [&](int set, int kt, int ks) {
         const int st = kt % NST;
 #pragma unroll
+        for (int x = 0; x < MT; ++x) {
+            ph[set][x] = frag(st, 0, wr * WM + 32 * x + (lane & 31), ks);
+            if constexpr (SPLIT) pl[set][x] = frag(st, PBYTES, wr * WM + 32 * x + (lane & 31), ks);
+        }
+#pragma unroll
+        for (int y = 0; y < NT; ++y) {
+            qh[set][y] = frag(st, NP * PBYTES, wc * WN + 32 * y + (lane & 31), ks);
+            if constexpr (SPLIT) ql[set][y] = frag(st, NP * PBYTES + QBYTES, wc * WN + 32 * y + (lane & 31), ks);
+        }
+    };
+    for (int kt = k0; kt < k0 + NST - 1 && kt < k1; ++kt) fill(kt);
+    stage_ready(k0);
+    load(0, k0, 0);
+    for (int kt = k0; kt < k1; ++kt) {
+#pragma unroll
         for (int ks = 0; ks < BK / 16; ++ks) {
-            h8 ph[MT], qh[NT], pl[SPLIT ? MT : 1], ql[SPLIT ? NT : 1];
-#pragma unroll
-            for (int x = 0; x < MT; ++x) {
-                ph[x] = frag(st, 0, wr * WM + 32 * x + (lane & 31), ks);
-                if constexpr (SPLIT) pl[x] = frag(st, PBYTES, wr * WM + 32 * x + (lane & 31), ks);
+            const int set = ks & 1;
+            if (ks + 1 < BK / 16) load(set ^ 1, kt, ks + 1);
+            else if (kt + 1 < k1) {
+                stage_ready(kt + 1);
+                load(set ^ 1, kt + 1, 0);
             }
-#pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                qh[y] = frag(st, NP * PBYTES, wc * WN + 32 * y + (lane & 31), ks);
-                if constexpr (SPLIT) ql[y] = frag(st, NP * PBYTES + QBYTES, wc * WN + 32 * y + (lane & 31), ks);
-            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int x = 0; x < MT; ++x)
 #pragma unroll
                 for (int y = 0; y < NT; ++y) {
-                    acc[x][y] = mfma(ph[x], qh[y], acc[x][y]);
                     if constexpr (SPLIT) {
-                        low[x][y] = mfma(ph[x], ql[y], low[x][y]);
-                        low[x][y] = mfma(pl[x], qh[y], low[x][y]);
+                        acc[x][y] = mfma(ph[set][x], ql[set][y], acc[x][y]);
+                        acc[x][y] = mfma(pl[set][x], qh[set][y], acc[x][y]);
                     }
+                    acc[x][y] = mfma(ph[set][x], qh[set][y], acc[x][y]);
                 }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (SPLIT && (((kt + 1) & (chunk - 1)) == 0 || kt + 1 == k1)) flush();      // chunk is a power of two
+        if (SPLIT && (((kt + 1) & (chunk - 1)) == 0 || kt + 1 == k1))      // chunk is a power of two
+#pragma unroll
+            for (int x = 0; x < MT; ++x)
+#pragma unroll
+                for (int y = 0; y < NT; ++y) {
+                    sum[SPLIT ? x : 0][SPLIT ? y : 0] += acc[x][y];
+                    acc[x][y] = f32x16{};
+                }
     }
     if constexpr (SPLIT)
 #pragma unroll
@@ -793,9 +811,9 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                         v[z] *= S;
                     }
                 } else if constexpr (KIND == B_OF_A) {
-                    const h4 rh = *reinterpret_cast<const h4*>(R + (long)c * l.mp + row0);       // R is symmetric
+                    const h4 rh = *reinterpret_cast<const h4*>(R + place(l.mp, c, row0));       // R is symmetric
                     h4 rl = {};
-                    if constexpr (SPLIT) rl = *reinterpret_cast<const h4*>(R + pp + (long)c * l.mp + row0);
+                    if constexpr (SPLIT) rl = *reinterpret_cast<const h4*>(R + pp + place(l.mp, c, row0));
                     const float dc = dv[c];
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
@@ -809,14 +827,14 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                     const float alpha = xi * INV_S;
                     const long plane = (long)l.mp * l.np;
                     if (!swap) {                        // rows are i, columns j
-                        const h4 xh = *reinterpret_cast<const h4*>(xt + (long)c * l.mp + row0), xl = *reinterpret_cast<const h4*>(xt + plane + (long)c * l.mp + row0);
+                        const h4 xh = *reinterpret_cast<const h4*>(xt + place(l.np, c, row0)), xl = *reinterpret_cast<const h4*>(xt + plane + place(l.np, c, row0));
 #pragma unroll
                         for (int z = 0; z < 4; ++z) v[z] = fmaf(ev[row0 + z], ((float)xh[z] + (float)xl[z]) * xi, v[z] * alpha);
                     } else {
                         const float ec = ev[c];
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            const long o = (long)(row0 + z) * l.mp + c;
+                            const long o = place(l.np, row0 + z, c);
                             v[z] = fmaf(ec, ((float)xt[o] + (float)xt[plane + o]) * xi, v[z] * alpha);
                         }
                     }
@@ -844,14 +862,15 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
     // ---- the tile and its transpose, hi and lo, through LDS: 16-byte stores of whole rows
     _Float16* stage = reinterpret_cast<_Float16*>(lds);
     _Float16 *out, *outt;
-    long ld, ldt, plane;
+    long plane;
+    int onr, ort;                                       // rows of the planes that are written
     constexpr int planes = (KIND == X_NEXT || SPLIT) ? 2 : 1;
     if constexpr (KIND == X_NEXT) {
         out = reinterpret_cast<_Float16*>(ws + of.x); outt = reinterpret_cast<_Float16*>(ws + of.xt(a.k + 1));
-        ld = l.np; ldt = l.mp; plane = (long)l.mp * l.np;
+        onr = l.mp; ort = l.np; plane = (long)l.mp * l.np;
     } else {
         out = outt = reinterpret_cast<_Float16*>(ws + (KIND == A_OF_X ? of.r : of.b));
-        ld = ldt = l.mp; plane = (long)l.mp * l.mp;
+        onr = ort = l.mp; plane = (long)l.mp * l.mp;
     }
 #pragma unroll
     for (int pl = 0; pl < planes; ++pl)
@@ -886,15 +905,14 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                     }
             __syncthreads();
             _Float16* o = (tr ? outt : out) + pl * plane;
-            const long lo = tr ? ldt : ld;
-            const int r0 = tr ? tj * TN : ti * TM, c0 = tr ? ti * TM : tj * TN;
+            const int r0 = tr ? tj * TN : ti * TM, c0 = tr ? ti * TM : tj * TN, of_rows = tr ? ort : onr;
             // what lies beyond an odd number of 128s is not stored
-            const int nr = tr ? TN : rows < TM ? rows : TM, nc = tr ? (rows < TM ? rows : TM) : TN;
-            const int pitch = tr ? TM + 8 : TN + 8, per_row = (tr ? TM : TN) / 8;
+            const int height = tr ? TN : TM, nr = tr ? TN : rows < TM ? rows : TM, nc = tr ? (rows < TM ? rows : TM) : TN;
+            const int pitch = tr ? TM + 8 : TN + 8;
             for (int w = threadIdx.x; w < TM * TN / 8; w += 256) {
-                const int r = w / per_row, c = w % per_row * 8;
+                const int r = (w >> 2) % height, c = (w >> 2) / height * 32 + (w & 3) * 8;        // along a block of 32 columns
                 if (TM == TN || (r < nr && c < nc))
-                    *reinterpret_cast<uint4*>(o + (long)(r0 + r) * lo + c0 + c) = *reinterpret_cast<const uint4*>(stage + r * pitch + c);
+                    *reinterpret_cast<uint4*>(o + place(of_rows, r0 + r, c0 + c)) = *reinterpret_cast<const uint4*>(stage + r * pitch + c);
             }
             __syncthreads();
         }
