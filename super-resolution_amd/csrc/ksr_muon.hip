@@ -402,13 +402,13 @@ __global__ void __launch_bounds__(512) ns_small_kernel(Mats p) {
 // ================================================================================================ large matrices
 // All matrices of a call that are not small run together, whatever their shapes: per step one launch for A, one for B and one for
 // the next X, over the tiles of all of them.
-// Layout of every plane: blocks of 32 columns, row after row within a block, so that 16 rows of a block are 1 KB without a gap:
-// the products are bound by their loads from the L2, and rows of 64 or 128 bytes a pitch apart reach two thirds of the rate.
+// Layout of every plane: blocks of 32 columns, row after row within a block, so that 16 rows of a block are 1 KB without a gap: the
+// products are bound by their loads from the L2 (2 x 2048 x 2048 fp32: 1530 us with whole rows, 1470 us with blocks).
 // Buffers of one matrix, padded to the tile in both directions with zeros that every step reproduces (A, B and X of a zero row
 // or column are zero), so that no product needs a bounds check:  X [mp][np] and X^T [np][mp] (twice), R and B [mp][mp].  With X
 // in both orders each of the three products contracts the contiguous dimension of both operands.
 constexpr int MAX_LARGE = 24;
-constexpr int NORM_PARTS = 256;                         // partial sums of squares per matrix, at most
+constexpr int NORM_PARTS = 1024;                         // partial sums of squares per matrix, at most
 constexpr int CUS = 256, SLOTS = 1024;                  // SLOTS: partial tiles of the products that are cut along k, at most
 
 struct LMat {
@@ -502,6 +502,7 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(LargeArgs a) {
                 for (int z = 0; z < 4; ++z) s = fma((double)u[z], (double)u[z], s);
             }
         } else {
+#pragma unroll 4
             for (int i = x0; i < cols; i += tx) {
                 const double u = load_u<MODE, true>(a.s, mt, sub, by_col ? o : i, by_col ? i : o);
                 s = fma(u, u, s);
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(LargeArgs a) {
 template <int MODE, bool SPLIT>
 __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
     __shared__ _Float16 tile[2][64][72];
-    __shared__ double part[NORM_PARTS];
+    __shared__ double part[4];
     int q = 0;
     while (q + 1 < a.l.count && (int)blockIdx.y >= a.l.e[q + 1].first) ++q;
     const LMat& le = a.l.e[q];
@@ -533,20 +534,31 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
     if ((int)blockIdx.x >= ni * nj) return;
     const Offsets of(le.mp, le.np, SPLIT);
     char* ws = a.l.ws + le.off + at * of.per;
-    if ((int)threadIdx.x < le.parts) part[threadIdx.x] = reinterpret_cast<const double*>(ws + of.sq)[threadIdx.x];
-    __syncthreads();
+    // the tile's values are on their way while the norm is added up
+    const int i0 = (int)blockIdx.x / nj * 64, j0 = (int)blockIdx.x % nj * 64;
+    const bool across = (mt.cs <= mt.rs) != (le.tall != 0);             // whether columns of X are contiguous in U
+    float u[16];
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        const int t = (int)threadIdx.x + 256 * w, i = i0 + (across ? t >> 6 : t & 63), j = j0 + (across ? t & 63 : t >> 6);
+        const int ic = i < le.m ? i : le.m - 1, jc = j < le.n ? j : le.n - 1;
+        u[w] = load_u<MODE, false>(a.s, mt, sub, le.tall ? jc : ic, le.tall ? ic : jc);
+        u[w] = i < le.m && j < le.n ? u[w] : 0.f;
+    }
     double total = 0;
-    for (int i = 0; i < le.parts; ++i) total += part[i];
+    for (int i = threadIdx.x; i < le.parts; i += 256) total += reinterpret_cast<const double*>(ws + of.sq)[i];
+    total = wave_sum(total);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = total;
+    __syncthreads();
+    total = part[0] + part[1] + part[2] + part[3];
     int e;
     const float xi0 = scales(a.s, total, e);
     if (blockIdx.x == 0 && (int)threadIdx.x <= a.s.steps)
         reinterpret_cast<float*>(ws + of.xi)[threadIdx.x] = threadIdx.x == 0 ? xi0 : scale_at(a.s, log_norm(a.s, total), (int)threadIdx.x);
-    const int i0 = (int)blockIdx.x / nj * 64, j0 = (int)blockIdx.x % nj * 64;
-    const bool across = (mt.cs <= mt.rs) != (le.tall != 0);             // whether columns of X are contiguous in U
-    for (int t = threadIdx.x; t < 4096; t += 256) {
-        const int i = across ? t >> 6 : t & 63, j = across ? t & 63 : t >> 6, gi = i0 + i, gj = j0 + j;
-        float v = 0.f;
-        if (gi < le.m && gj < le.n) v = scaled(load_u<MODE, false>(a.s, mt, sub, le.tall ? gj : gi, le.tall ? gi : gj), e);
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        const int t = (int)threadIdx.x + 256 * w, i = across ? t >> 6 : t & 63, j = across ? t & 63 : t >> 6;
+        const float v = scaled(u[w], e);
         const _Float16 hi = (_Float16)v;
         tile[0][i][j] = hi;
         tile[1][i][j] = (_Float16)(v - (float)hi);
@@ -569,9 +581,13 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
 //   B_OF_A      P = Q = R, tiles of the lower triangle:   B - diag B, e = a + diag B
 //   X_NEXT      P = B, Q = X^T:                            X, X^T
 //   X_LAST      the same, result or weight update; TALL: P = X^T, Q = B, so that lanes run along U's rows either way
-// Four waves, each (TILE / 2)^2 of the TILE^2 outputs; NST stages of BK columns of P and Q in LDS, filled by LDS-DMA ahead of
-// their use.  Rows of a stage hold 16-byte chunks in an order that depends on the row (chunk c of row r at c ^ f(r)), so that the
-// eight lanes that read at once hit all banks.
+// Workgroups of TM x TN outputs, each wave WM x WN of them; NST stages of BK columns of P and Q in LDS, filled by LDS-DMA ahead of
+// their use.  What bounds the products is that traffic from the L2 and the MALL (4096 x 4096, X in 128 x 128 tiles: 178 us; 157 us
+// without the matrix instructions, 111 us without the loads), so X, which has no triangle to lose, takes the largest tiles that
+// LDS and registers hold, eight waves each: 256 x 256 (164 us; 256 x 128 in four waves: 179 us), SPLIT 256 x 128 (120 us for
+// 2 x 2048; 128 x 128: 123 us).  A and B stay at 128 x 128, in two stages of 64 columns: 102 and 111 us (four of 32: 110 and 119 us).
+// Rows of a stage hold 16-byte chunks in an order that depends on the row (chunk c of row r at c ^ f(r)), so that the eight lanes
+// that read at once hit all banks.
 // Sums: along k in chunks of `chunk_of` columns; a chunk's sum is added to the tile's in the order of k.  Shorter chains of
 // roundings, and the result does not depend on who computes which chunk:
 // Work split: of T tiles the first `whole` = 256 floor(T / 256) have a workgroup each; each chunk of the others has one of its
@@ -586,22 +602,30 @@ __host__ __device__ inline int chunk_of(int k) {
     return c;
 }
 
-// tiles of a product: of the lower triangle, or of X (U, transposed or not) with the last row of tiles possibly cut off
+// tiles of a product: of the lower triangle (tiles TM / TN times as high as wide: block column tj <= (ti + 1) TM / TN - 1), or of X
+// (of U, transposed or not).  The last row of tiles may be cut off.
 template <int TM, int TN, int KIND> __host__ __device__ inline int tiles_of(const LMat& e) {
-    if (KIND == A_OF_X || KIND == B_OF_A) return e.mp / TM * (e.mp / TM + 1) / 2;
+    constexpr int Q = TM / TN;
+    if (KIND == A_OF_X || KIND == B_OF_A) {
+        const int nt = e.mp / TN, mt = nt / Q;                         // whole rows of tiles, and nt % Q blocks below them
+        return Q * mt * (mt + 1) / 2 + (nt % Q ? nt : 0);
+    }
     const bool swap = KIND == X_LAST && e.tall;
-    return ((swap ? e.np : e.mp) + TM - 1) / TM * ((swap ? e.mp : e.np) / TN);
+    return ((swap ? e.np : e.mp) + TM - 1) / TM * (((swap ? e.mp : e.np) + TN - 1) / TN);
 }
 
-template <int TM, int TN, int BK, int NST, bool SPLIT, int KIND>
-__global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
-    constexpr int NP = SPLIT ? 2 : 1, WM = TM / 2, WN = TN / 2, MT = WM / 32, NT = WN / 32, CH = BK / 8;
+template <int TM, int TN, int WM, int WN, int BK, int NST, bool SPLIT, int KIND>
+__global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) == 4 ? 2 : 1) ns_gemm_kernel(LargeArgs a) {
+    constexpr int WC = TN / WN, WAVES = TM / WM * WC, TH = 64 * WAVES;
+    constexpr int NP = SPLIT ? 2 : 1, MT = WM / 32, NT = WN / 32, CH = BK / 8;
+    constexpr bool ODD = TM > 128 || TN > 128;                          // buffers are padded to 128: the last tile may be cut off
     constexpr int PBYTES = TM * BK * 2, QBYTES = TN * BK * 2, STAGE = NP * (PBYTES + QBYTES);
-    static_assert(NST * STAGE >= TM * (TN + 8) * 2 && NST * STAGE >= TN * (TM + 8) * 2, "the output tile reuses the stages");
-    static_assert((KIND != A_OF_X && KIND != B_OF_A) || TM == TN, "the triangle's tiles are square");
+    constexpr int HALVES = NST * STAGE >= TM * (TN + 8) * 2 && NST * STAGE >= TN * (TM + 8) * 2 ? 1 : 2;      // the output tile reuses the stages
+    static_assert(NST * STAGE >= TM / HALVES * (TN + 8) * 2 && NST * STAGE >= TN * (TM / HALVES + 8) * 2 && TM / HALVES >= WM, "output tile");
+    static_assert(TM % TN == 0, "tiles_of");
     __shared__ __attribute__((aligned(16))) char lds[NST * STAGE];
     __shared__ int arrived;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave >> 1, wc = wave & 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / WC, wc = wave % WC;
     constexpr bool SYM = KIND == A_OF_X || KIND == B_OF_A;
     int t, slice = 0, slices = 1, slot = 0, q = 0;      // slot: of the tile's first partial sums
     if ((int)blockIdx.x < a.whole) {
@@ -629,17 +653,19 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
     const LMat& l = a.l.e[q];
     t -= SYM ? l.sym : l.full[KIND == X_LAST];
     const bool swap = KIND == X_LAST && l.tall;
-    const int mt = (swap ? l.np + TM - 1 : l.mp + TM - 1) / TM, nt = (swap ? l.mp : l.np) / TN, per = SYM ? mt * (mt + 1) / 2 : mt * nt;
+    const int mt = ((swap ? l.np : l.mp) + TM - 1) / TM, per = tiles_of<TM, TN, KIND>(l);
     const int at = t / per, sub = l.sub0 + at;
     t -= at * per;
     const Offsets of(l.mp, l.np, SPLIT);
     char* ws = a.l.ws + l.off + at * of.per;
     int ti, tj;
-    if constexpr (SYM) {
-        ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-        while (ti * (ti + 1) / 2 > t) --ti;
-        tj = t - ti * (ti + 1) / 2;
+    if constexpr (SYM) {                                // Q (ti + 1) tiles in row ti
+        constexpr int Q = TM / TN;
+        const int u = t / Q;
+        ti = (int)((sqrtf(8.f * (float)u + 1.f) - 1.f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= u) ++ti;
+        while (ti * (ti + 1) / 2 > u) --ti;
+        tj = t - Q * (ti * (ti + 1) / 2);
     } else { ti = t % mt; tj = t / mt; }
     const _Float16* R = reinterpret_cast<const _Float16*>(ws + of.r);
     const _Float16* xt = reinterpret_cast<const _Float16*>(ws + of.xt(a.k));
@@ -658,9 +684,10 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
     }
     P += (long)ti * TM * 32;
     Q += (long)tj * TN * 32;
-    const int rows = SYM ? TM : (swap ? l.np : l.mp) - ti * TM;        // of P; fewer than TM in the last tile of an odd number of 128s
+    // rows of P and Q that exist: fewer than the tile's in the last one of an odd number of 128s
+    const int rows = pr - ti * TM, cols = qr - tj * TN;
     // LDS-DMA: one instruction of a wave brings 64 chunks of 16 bytes; lane -> (row, slot), the chunk that belongs there
-    constexpr int ROWS = 64 / CH, PI = TM / ROWS / 4, QI = TN / ROWS / 4;        // rows per instruction, instructions per wave and plane
+    constexpr int ROWS = 64 / CH, PI = TM / ROWS / WAVES, QI = TN / ROWS / WAVES;        // rows per instruction, instructions per wave and plane
     constexpr int PER_STAGE = NP * (PI + QI);                           // a wave's instructions per stage
     const int drow = lane / CH, dslot = lane % CH;
     auto f = [](int row) { return CH == 8 ? (row & 7) : ((row >> 1) & 3); };
@@ -671,13 +698,13 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
 #pragma unroll
             for (int i = 0; i < PI; ++i) {
                 const int row = (wave * PI + i) * ROWS + drow;
-                const _Float16* src = P + pl * pp + place(pr, TM == TN || row < rows ? row : 0, kt * BK + 8 * (dslot ^ f(row)));
+                const _Float16* src = P + pl * pp + place(pr, !ODD || row < rows ? row : 0, kt * BK + 8 * (dslot ^ f(row)));
                 ksr_dma16<false>(src, to + pl * PBYTES + (wave * PI + i) * 1024);
             }
 #pragma unroll
             for (int i = 0; i < QI; ++i) {
                 const int row = (wave * QI + i) * ROWS + drow;
-                const _Float16* src = Q + pl * qp + place(qr, row, kt * BK + 8 * (dslot ^ f(row)));
+                const _Float16* src = Q + pl * qp + place(qr, TN <= 128 || row < cols ? row : 0, kt * BK + 8 * (dslot ^ f(row)));
                 ksr_dma16<false>(src, to + NP * PBYTES + pl * QBYTES + (wave * QI + i) * 1024);
             }
         }
@@ -761,7 +788,7 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
             for (int y = 0; y < NT; ++y)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    __hip_atomic_store(own + ((x * NT + y) * 16 + r) * 256, acc[x][y][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(own + ((x * NT + y) * 16 + r) * TH, acc[x][y][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         // Device-scope accesses go past the caches of the eight dies, and a wave's are complete when its count of outstanding ones
         // is 0: the sums are in place before the arrival is counted.  (A release fence would write back a whole L2 per workgroup.)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -781,7 +808,7 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                 for (int y = 0; y < NT; ++y)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        acc[x][y][r] += __hip_atomic_load(part + (long)w * TM * TN + ((x * NT + y) * 16 + r) * 256, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        acc[x][y][r] += __hip_atomic_load(part + (long)w * TM * TN + ((x * NT + y) * 16 + r) * TH, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     ksr_lds_barrier();                                  // LDS is free for the output tile
     // ---- values
@@ -811,6 +838,7 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                         v[z] *= S;
                     }
                 } else if constexpr (KIND == B_OF_A) {
+                    if (ODD && row0 - ti * TM >= rows) continue;
                     const h4 rh = *reinterpret_cast<const h4*>(R + place(l.mp, c, row0));       // R is symmetric
                     h4 rl = {};
                     if constexpr (SPLIT) rl = *reinterpret_cast<const h4*>(R + pp + place(l.mp, c, row0));
@@ -823,7 +851,7 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                             v[z] = 0.f;
                         } else v[z] = S * (sp.b * r + sp.c * ((di + dc) * r + sq));
                     }
-                } else if (TM == TN || row0 - ti * TM < rows) {
+                } else if (!ODD || (row0 - ti * TM < rows && c - tj * TN < cols)) {
                     const float alpha = xi * INV_S;
                     const long plane = (long)l.mp * l.np;
                     if (!swap) {                        // rows are i, columns j
@@ -856,7 +884,7 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
                 }
 #pragma unroll
                 for (int z = 0; z < 4; ++z) acc[x][y][4 * g + z] = v[z];
-                if (TM != TN && g == 3) __builtin_amdgcn_sched_barrier(0);        // more of X^T in flight would spill
+                if (ODD && g == 3) __builtin_amdgcn_sched_barrier(0);        // more of X^T in flight would spill
             }
     if constexpr (KIND == X_LAST) return;
     // ---- the tile and its transpose, hi and lo, through LDS: 16-byte stores of whole rows
@@ -876,45 +904,55 @@ __global__ void __launch_bounds__(256, 2) ns_gemm_kernel(LargeArgs a) {
     for (int pl = 0; pl < planes; ++pl)
 #pragma unroll
         for (int tr = 0; tr < 2; ++tr) {
-            if (tr == 1 && KIND != X_NEXT && ti == tj) continue;
             if (tr == 0 && pl == 1 && !SPLIT) continue;              // X's lo is only read through X^T (the linear term)
-            if constexpr (TM != TN)                                  // nothing rounded is kept for the next round: it would spill
 #pragma unroll
-                for (int x = 0; x < MT; ++x)
+            for (int half = 0; half < HALVES; ++half) {
+                constexpr int HM = TM / HALVES;                      // rows of the tile in LDS at a time
+                if constexpr (ODD)                                       // nothing rounded is kept for the next round: it would spill
 #pragma unroll
-                    for (int y = 0; y < NT; ++y) asm volatile("" : "+v"(acc[x][y]));
+                    for (int x = 0; x < MT; ++x)
 #pragma unroll
-            for (int x = 0; x < MT; ++x)
+                        for (int y = 0; y < NT; ++y) asm volatile("" : "+v"(acc[x][y]));
+                if (HALVES == 1 || wr * WM / HM == half)
 #pragma unroll
-                for (int y = 0; y < NT; ++y)
+                    for (int x = 0; x < MT; ++x)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int r = wr * WM + 32 * x + 8 * g + 4 * (lane >> 5), c = wc * WN + 32 * y + (lane & 31);
-                        h4 w;
+                        for (int y = 0; y < NT; ++y)
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const float v = acc[x][y][4 * g + z];
-                            const _Float16 hi = (_Float16)v;
-                            w[z] = pl ? (_Float16)(v - (float)hi) : hi;
-                        }
-                        if (tr) *reinterpret_cast<h4*>(stage + c * (TM + 8) + r) = w;
-                        else {
+                            for (int g = 0; g < 4; ++g) {
+                                const int r = wr * WM - half * HM + 32 * x + 8 * g + 4 * (lane >> 5), c = wc * WN + 32 * y + (lane & 31);
+                                h4 w;
 #pragma unroll
-                            for (int z = 0; z < 4; ++z) stage[(r + z) * (TN + 8) + c] = w[z];
-                        }
+                                for (int z = 0; z < 4; ++z) {
+                                    const float v = acc[x][y][4 * g + z];
+                                    const _Float16 hi = (_Float16)v;
+                                    w[z] = pl ? (_Float16)(v - (float)hi) : hi;
+                                }
+                                if (tr) *reinterpret_cast<h4*>(stage + c * (HM + 8) + r) = w;
+                                else {
+#pragma unroll
+                                    for (int z = 0; z < 4; ++z) stage[(r + z) * (TN + 8) + c] = w[z];
+                                }
+                            }
+                __syncthreads();
+                _Float16* o = (tr ? outt : out) + pl * plane;
+                const int i0 = ti * TM + half * HM, j0 = tj * TN, of_rows = tr ? ort : onr;
+                constexpr int PITCH_N = TN + 8, PITCH_M = HM + 8;
+                const int height = tr ? TN : HM, pitch = tr ? PITCH_M : PITCH_N;
+                for (int w = threadIdx.x; w < HM * TN / 8; w += TH) {
+                    const int r = (w >> 2) % height, c = (w >> 2) / height * 32 + (w & 3) * 8;        // along a block of 32 columns
+                    const int i = tr ? c : r, j = tr ? r : c;        // row and column of the product's tile
+                    // what lies beyond an odd number of 128s is not stored; of a symmetric product, nothing above the diagonal's
+                    // blocks of TN, and the transposes of those below it
+                    bool ok = !ODD || (half * HM + i < rows && j < cols);
+                    if constexpr (SYM) {
+                        const int bi = (i0 + i) / TN;
+                        ok = ok && (tr ? bi > tj : bi >= tj);
                     }
-            __syncthreads();
-            _Float16* o = (tr ? outt : out) + pl * plane;
-            const int r0 = tr ? tj * TN : ti * TM, c0 = tr ? ti * TM : tj * TN, of_rows = tr ? ort : onr;
-            // what lies beyond an odd number of 128s is not stored
-            const int height = tr ? TN : TM, nr = tr ? TN : rows < TM ? rows : TM, nc = tr ? (rows < TM ? rows : TM) : TN;
-            const int pitch = tr ? TM + 8 : TN + 8;
-            for (int w = threadIdx.x; w < TM * TN / 8; w += 256) {
-                const int r = (w >> 2) % height, c = (w >> 2) / height * 32 + (w & 3) * 8;        // along a block of 32 columns
-                if (TM == TN || (r < nr && c < nc))
-                    *reinterpret_cast<uint4*>(o + place(of_rows, r0 + r, c0 + c)) = *reinterpret_cast<const uint4*>(stage + r * pitch + c);
+                    if (ok) *reinterpret_cast<uint4*>(o + place(of_rows, (tr ? j0 : i0) + r, (tr ? i0 : j0) + c)) = *reinterpret_cast<const uint4*>(stage + r * pitch + c);
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
 }
 
@@ -931,8 +969,8 @@ long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& s
     l.count = 0;
     l.split = split;
     for (int pass = 0; pass < 2; ++pass) {
-        // the tile: 128 where that gives at least 128 tiles of X (the wide tile's products run at 1.5 times the rate of the
-        // narrow one's; a chip that is half empty costs more)
+        // the tile: 128 where that gives at least 128 tiles of X.  A wide tile reads less, many narrow ones fill the chip: 25 matrices
+        // with 384 wide tiles take 697 us so and 730 us with the narrow ones; 777 x 2051 (119 wide tiles) is latency, 266 us narrow
         l.tile = pass == 0 ? 128 : 64;
         l.count = 0;
         entry = entry0;
@@ -961,7 +999,7 @@ long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& s
             e.nsub = left < room ? left : (int)room;
             e.sub0 = sub;
             const long elements = (long)e.m * e.n;
-            e.parts = elements / 8192 < 1 ? 1 : elements / 8192 < NORM_PARTS ? (int)(elements / 8192) : NORM_PARTS;
+            e.parts = elements / 4096 < 1 ? 1 : elements / 4096 < NORM_PARTS ? (int)(elements / 4096) : NORM_PARTS;
             e.off = off;
             e.first = matrices;
             m[l.count++] = Mat{k.src, k.dst, k.momentum, (long)k.row_stride, (long)k.col_stride, (long)k.batch_stride, k.rows, k.cols, k.batch, 0};
@@ -1007,7 +1045,7 @@ template <int MODE, bool SPLIT> void start_large(const LargeArgs& a, hipStream_t
     hipLaunchKernelGGL((ns_prepare_kernel<MODE, SPLIT>), dim3(tiles, matrices), dim3(256), 0, st, a);
 }
 
-template <int TM, int TN, int BK, int NST, bool SPLIT, int KIND> void product(LargeArgs& a, hipStream_t st) {
+template <int TM, int TN, int WM, int WN, int BK, int NST, bool SPLIT, int KIND> void product(LargeArgs& a, hipStream_t st) {
     constexpr bool SYM = KIND == A_OF_X || KIND == B_OF_A;
     int tiles = 0;
     for (int i = 0; i < a.l.count; ++i) {
@@ -1023,8 +1061,10 @@ template <int TM, int TN, int BK, int NST, bool SPLIT, int KIND> void product(La
         const int ch = chunk_of(KIND == A_OF_X ? e.n : e.m), kp = KIND == A_OF_X ? e.np : e.mp;
         if (n > 0) cut += (long)n * ((kp + ch - 1) / ch);
     }
-    a.cut = cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile;
-    hipLaunchKernelGGL((ns_gemm_kernel<TM, TN, BK, NST, SPLIT, KIND>), dim3((unsigned)(a.cut ? a.whole + cut : tiles)), dim3(256), 0, st, a);
+    // Cut only what is worth its traffic: four chunks or more, or fewer tiles than CUs (429 tiles of 832 columns in two chunks: 20 us,
+    // uncut 14 us)
+    a.cut = cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile && (tiles < CUS || cut >= 4l * (tiles - a.whole));
+    hipLaunchKernelGGL((ns_gemm_kernel<TM, TN, WM, WN, BK, NST, SPLIT, KIND>), dim3((unsigned)(a.cut ? a.whole + cut : tiles)), dim3(TM / WM * (TN / WN) * 64), 0, st, a);
 }
 
 template <int TILE, bool SPLIT> int run_large(LargeArgs& a, hipStream_t st) {
@@ -1033,14 +1073,25 @@ template <int TILE, bool SPLIT> int run_large(LargeArgs& a, hipStream_t st) {
     else if (mode == BF16) start_large<BF16, SPLIT>(a, st);
     else start_large<MUON, SPLIT>(a, st);
     KSR_LAUNCH_CHECK("muon_batch");
-    constexpr int BK = SPLIT ? 32 : 64, NST = TILE == 64 ? 4 : 2;
-    constexpr bool WIDE = TILE == 128 && !SPLIT;       // X in 256 x 128: a wave's 128 x 64 needs 3/4 of the LDS reads per product
-    constexpr int XM = WIDE ? 256 : TILE, XK = WIDE ? 32 : BK, XS = WIDE ? 3 : NST;
     for (a.k = 0; a.k < a.s.steps; ++a.k) {
-        product<TILE, TILE, BK, NST, SPLIT, A_OF_X>(a, st);
-        product<TILE, TILE, BK, NST, SPLIT, B_OF_A>(a, st);
-        if (a.k + 1 < a.s.steps) product<XM, TILE, XK, XS, SPLIT, X_NEXT>(a, st);
-        else product<XM, TILE, XK, XS, SPLIT, X_LAST>(a, st);
+        const bool last = a.k + 1 == a.s.steps;
+        if constexpr (TILE == 64) {
+            constexpr int BK = SPLIT ? 32 : 64;
+            product<64, 64, 32, 32, BK, 4, SPLIT, A_OF_X>(a, st);
+            product<64, 64, 32, 32, BK, 4, SPLIT, B_OF_A>(a, st);
+            if (last) product<64, 64, 32, 32, BK, 4, SPLIT, X_LAST>(a, st);
+            else product<64, 64, 32, 32, BK, 4, SPLIT, X_NEXT>(a, st);
+        } else if constexpr (SPLIT) {
+            product<128, 128, 64, 64, 32, 2, true, A_OF_X>(a, st);
+            product<128, 128, 64, 64, 32, 2, true, B_OF_A>(a, st);
+            if (last) product<256, 128, 64, 64, 32, 3, true, X_LAST>(a, st);
+            else product<256, 128, 64, 64, 32, 3, true, X_NEXT>(a, st);
+        } else {
+            product<128, 128, 64, 64, 64, 2, false, A_OF_X>(a, st);
+            product<128, 128, 64, 64, 64, 2, false, B_OF_A>(a, st);
+            if (last) product<256, 256, 128, 64, 32, 4, false, X_LAST>(a, st);
+            else product<256, 256, 128, 64, 32, 4, false, X_NEXT>(a, st);
+        }
         KSR_LAUNCH_CHECK("muon_batch");
     }
     return KSR_OK;
