@@ -80,11 +80,13 @@ struct Apply {
         keep = 1.f - lr * s.wd;
         rate = lr * s.scale * sqrtf((float)(m.rows > m.cols ? m.rows : m.cols));
     }
-    template <int MODE> __device__ __forceinline__ void store(const Mat& m, long o, float v) const {
-        if constexpr (MODE == MUON) {
-            float* w = reinterpret_cast<float*>(m.dst) + o;
-            *w = fmaf(-rate, v, *w * keep);
-        } else if constexpr (MODE == BF16) reinterpret_cast<__bf16*>(m.dst)[o] = (__bf16)v;
+    // the weights of several results are read before the first is written: a load behind a store would wait for it
+    template <int MODE> __device__ __forceinline__ float old(const Mat& m, long o) const {
+        return MODE == MUON ? reinterpret_cast<const float*>(m.dst)[o] : 0.f;
+    }
+    template <int MODE> __device__ __forceinline__ void store(const Mat& m, long o, float v, float w) const {
+        if constexpr (MODE == MUON) reinterpret_cast<float*>(m.dst)[o] = fmaf(-rate, v, w * keep);
+        else if constexpr (MODE == BF16) reinterpret_cast<__bf16*>(m.dst)[o] = (__bf16)v;
         else reinterpret_cast<float*>(m.dst)[o] = v;
     }
 };
@@ -369,9 +371,19 @@ __device__ __forceinline__ void small_body(const Step& st, const Mat& mt, int su
                 if (last) {
                     const int j = 32 * (wave + 8 * s) + col;
 #pragma unroll
-                    for (int r = 0; r < 32; ++r) {
-                        const int i = 32 * (r >> 4) + acc_row(r & 15, lane);
-                        if (i < m && j < n) ap.store<MODE>(mt, ((long)sub * mt.rows + (tall ? j : i)) * mt.cols + (tall ? i : j), x[r >> 4][r & 15]);
+                    for (int t = 0; t < 2; ++t) {
+                        float w[16];
+                        auto place_of = [&](int i, int jj) { return ((long)sub * mt.rows + (tall ? jj : i)) * mt.cols + (tall ? i : jj); };
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int i = 32 * t + acc_row(r, lane);
+                            w[r] = ap.old<MODE>(mt, place_of(i < m ? i : m - 1, j < n ? j : n - 1));
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int i = 32 * t + acc_row(r, lane);
+                            if (i < m && j < n) ap.store<MODE>(mt, place_of(i, j), x[t][r], w[r]);
+                        }
                     }
                 } else {
 #pragma unroll
@@ -409,7 +421,7 @@ __global__ void __launch_bounds__(512) ns_small_kernel(Mats p) {
 // in both orders each of the three products contracts the contiguous dimension of both operands.
 constexpr int MAX_LARGE = 24;
 constexpr int NORM_PARTS = 1024;                         // partial sums of squares per matrix, at most
-constexpr int CUS = 256, SLOTS = 1024;                  // SLOTS: partial tiles of the products that are cut along k, at most
+constexpr int CUS = 256, SLOTS = 1024, COUNTERS = 4 * SLOTS;      // partial sums of products that are cut along k: room for SLOTS wide tiles
 
 struct LMat {
     long off;                       // of the first matrix's buffers in the workspace
@@ -420,7 +432,7 @@ struct LMat {
 };
 struct Large {
     char* ws;
-    long o_part;                    // fp32 partial tiles, then SLOTS counters
+    long o_part;                    // COUNTERS counters, then fp32 partial tiles
     int count, tile, split;
     LMat e[MAX_LARGE];
 };
@@ -530,7 +542,7 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
     const int at = (int)blockIdx.y - le.first, sub = le.sub0 + at;
     const int nj = le.np / 64, ni = le.mp / 64;
     if (blockIdx.x == 0 && blockIdx.y == 0)
-        for (int t = threadIdx.x; t < SLOTS; t += 256) reinterpret_cast<int*>(a.l.ws + a.l.o_part)[t] = 0;
+        for (int t = threadIdx.x; t < COUNTERS; t += 256) reinterpret_cast<int*>(a.l.ws + a.l.o_part)[t] = 0;
     if ((int)blockIdx.x >= ni * nj) return;
     const Offsets of(le.mp, le.np, SPLIT);
     char* ws = a.l.ws + le.off + at * of.per;
@@ -582,10 +594,8 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
 //   X_NEXT      P = B, Q = X^T:                            X, X^T
 //   X_LAST      the same, result or weight update; TALL: P = X^T, Q = B, so that lanes run along U's rows either way
 // Workgroups of TM x TN outputs, each wave WM x WN of them; NST stages of BK columns of P and Q in LDS, filled by LDS-DMA ahead of
-// their use.  What bounds the products is that traffic from the L2 and the MALL (4096 x 4096, X in 128 x 128 tiles: 178 us; 157 us
-// without the matrix instructions, 111 us without the loads), so X, which has no triangle to lose, takes the largest tiles that
-// LDS and registers hold, eight waves each: 256 x 256 (164 us; 256 x 128 in four waves: 179 us), SPLIT 256 x 128 (120 us for
-// 2 x 2048; 128 x 128: 123 us).  A and B stay at 128 x 128, in two stages of 64 columns: 102 and 111 us (four of 32: 110 and 119 us).
+// their use.  What bounds large products is that traffic from the L2 and the MALL (4096 x 4096, X in 128 x 128 tiles: 178 us; 157 us
+// without the matrix instructions, 111 us without the loads); of small ones a third is the epilogue, which few workgroups share.
 // Rows of a stage hold 16-byte chunks in an order that depends on the row (chunk c of row r at c ^ f(r)), so that the eight lanes
 // that read at once hit all banks.
 // Sums: along k in chunks of `chunk_of` columns; a chunk's sum is added to the tile's in the order of k.  Shorter chains of
@@ -602,14 +612,9 @@ __host__ __device__ inline int chunk_of(int k) {
     return c;
 }
 
-// tiles of a product: of the lower triangle (tiles TM / TN times as high as wide: block column tj <= (ti + 1) TM / TN - 1), or of X
-// (of U, transposed or not).  The last row of tiles may be cut off.
+// tiles of a product: of the lower triangle, or of X (of U, transposed or not; the last row and column of tiles may be cut off)
 template <int TM, int TN, int KIND> __host__ __device__ inline int tiles_of(const LMat& e) {
-    constexpr int Q = TM / TN;
-    if (KIND == A_OF_X || KIND == B_OF_A) {
-        const int nt = e.mp / TN, mt = nt / Q;                         // whole rows of tiles, and nt % Q blocks below them
-        return Q * mt * (mt + 1) / 2 + (nt % Q ? nt : 0);
-    }
+    if (KIND == A_OF_X || KIND == B_OF_A) return e.mp / TM * (e.mp / TM + 1) / 2;
     const bool swap = KIND == X_LAST && e.tall;
     return ((swap ? e.np : e.mp) + TM - 1) / TM * (((swap ? e.mp : e.np) + TN - 1) / TN);
 }
@@ -622,7 +627,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
     constexpr int PBYTES = TM * BK * 2, QBYTES = TN * BK * 2, STAGE = NP * (PBYTES + QBYTES);
     constexpr int HALVES = NST * STAGE >= TM * (TN + 8) * 2 && NST * STAGE >= TN * (TM + 8) * 2 ? 1 : 2;      // the output tile reuses the stages
     static_assert(NST * STAGE >= TM / HALVES * (TN + 8) * 2 && NST * STAGE >= TN * (TM / HALVES + 8) * 2 && TM / HALVES >= WM, "output tile");
-    static_assert(TM % TN == 0, "tiles_of");
+    static_assert(TM == TN || KIND == X_NEXT || KIND == X_LAST, "a triangle of square tiles");
     __shared__ __attribute__((aligned(16))) char lds[NST * STAGE];
     __shared__ int arrived;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / WC, wc = wave % WC;
@@ -659,13 +664,11 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
     const Offsets of(l.mp, l.np, SPLIT);
     char* ws = a.l.ws + l.off + at * of.per;
     int ti, tj;
-    if constexpr (SYM) {                                // Q (ti + 1) tiles in row ti
-        constexpr int Q = TM / TN;
-        const int u = t / Q;
-        ti = (int)((sqrtf(8.f * (float)u + 1.f) - 1.f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= u) ++ti;
-        while (ti * (ti + 1) / 2 > u) --ti;
-        tj = t - Q * (ti * (ti + 1) / 2);
+    if constexpr (SYM) {                                // ti + 1 tiles in row ti
+        ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+        while (ti * (ti + 1) / 2 > t) --ti;
+        tj = t - ti * (ti + 1) / 2;
     } else { ti = t % mt; tj = t / mt; }
     const _Float16* R = reinterpret_cast<const _Float16*>(ws + of.r);
     const _Float16* xt = reinterpret_cast<const _Float16*>(ws + of.xt(a.k));
@@ -780,7 +783,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
             for (int y = 0; y < NT; ++y) acc[x][y] = sum[x][y];
     if (slices > 1) {
         int* counter = reinterpret_cast<int*>(a.l.ws + a.l.o_part) + slot;
-        float* part = reinterpret_cast<float*>(a.l.ws + a.l.o_part + 4l * SLOTS) + (long)slot * TM * TN + threadIdx.x;
+        float* part = reinterpret_cast<float*>(a.l.ws + a.l.o_part + 4l * COUNTERS) + (long)slot * TM * TN + threadIdx.x;
         float* own = part + (long)slice * TM * TN;
 #pragma unroll
         for (int x = 0; x < MT; ++x)
@@ -823,7 +826,17 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
 #pragma unroll
     for (int x = 0; x < MT; ++x)
 #pragma unroll
-        for (int y = 0; y < NT; ++y)
+        for (int y = 0; y < NT; ++y) {
+            float w[KIND == X_LAST ? 16 : 1];
+            if constexpr (KIND == X_LAST)
+                if (mode == MUON) {
+                    const int c = tj * TN + wc * WN + 32 * y + (lane & 31), cc = c < mat.cols ? c : mat.cols - 1;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = ti * TM + wr * WM + 32 * x + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+                        w[i] = ap.old<MUON>(mat, ((long)sub * mat.rows + (r < mat.rows ? r : mat.rows - 1)) * mat.cols + cc);
+                    }
+                }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int row0 = ti * TM + wr * WM + 32 * x + 8 * g + 4 * (lane >> 5), c = tj * TN + wc * WN + 32 * y + (lane & 31);
@@ -872,9 +885,9 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                             const int r = row0 + z;     // rows and columns of the result are those of U either way
                             if (r < mat.rows && c < mat.cols) {
                                 const long o = ((long)sub * mat.rows + r) * mat.cols + c;
-                                if (mode == F32) ap.store<F32>(mat, o, v[z]);
-                                else if (mode == BF16) ap.store<BF16>(mat, o, v[z]);
-                                else ap.store<MUON>(mat, o, v[z]);
+                                if (mode == F32) ap.store<F32>(mat, o, v[z], 0.f);
+                                else if (mode == BF16) ap.store<BF16>(mat, o, v[z], 0.f);
+                                else ap.store<MUON>(mat, o, v[z], w[KIND == X_LAST ? 4 * g + z : 0]);
                             }
                         }
                     } else {
@@ -886,6 +899,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                 for (int z = 0; z < 4; ++z) acc[x][y][4 * g + z] = v[z];
                 if (ODD && g == 3) __builtin_amdgcn_sched_barrier(0);        // more of X^T in flight would spill
             }
+        }
     if constexpr (KIND == X_LAST) return;
     // ---- the tile and its transpose, hi and lo, through LDS: 16-byte stores of whole rows
     _Float16* stage = reinterpret_cast<_Float16*>(lds);
@@ -934,7 +948,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                                     for (int z = 0; z < 4; ++z) stage[(r + z) * (TN + 8) + c] = w[z];
                                 }
                             }
-                __syncthreads();
+                ksr_lds_barrier();                                       // stores of the tile stay in flight across it
                 _Float16* o = (tr ? outt : out) + pl * plane;
                 const int i0 = ti * TM + half * HM, j0 = tj * TN, of_rows = tr ? ort : onr;
                 constexpr int PITCH_N = TN + 8, PITCH_M = HM + 8;
@@ -951,7 +965,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                     }
                     if (ok) *reinterpret_cast<uint4*>(o + place(of_rows, (tr ? j0 : i0) + r, (tr ? i0 : j0) + c)) = *reinterpret_cast<const uint4*>(stage + r * pitch + c);
                 }
-                __syncthreads();
+                ksr_lds_barrier();
             }
         }
 }
@@ -969,8 +983,8 @@ long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& s
     l.count = 0;
     l.split = split;
     for (int pass = 0; pass < 2; ++pass) {
-        // the tile: 128 where that gives at least 128 tiles of X.  A wide tile reads less, many narrow ones fill the chip: 25 matrices
-        // with 384 wide tiles take 697 us so and 730 us with the narrow ones; 777 x 2051 (119 wide tiles) is latency, 266 us narrow
+        // the tile: 128 where that gives at least 128 tiles of X.  A wide tile reads less, many narrow ones fill the chip: 12 matrices
+        // with 466 wide tiles: X 42 us so and 61 us with narrow ones; 777 x 2051 (119 wide tiles) is latency, 14 us narrow
         l.tile = pass == 0 ? 128 : 64;
         l.count = 0;
         entry = entry0;
@@ -1012,7 +1026,7 @@ long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& s
         l.o_part = off;
         if (pass == 1 || full >= 128) break;
     }
-    return l.o_part + 4l * SLOTS + 4l * SLOTS * l.tile * l.tile;
+    return l.o_part + 4l * COUNTERS + 4l * SLOTS * l.tile * l.tile;
 }
 
 // Largest singular value that each step can reach from [0, 1], and that A and B stay inside f16's range
@@ -1062,36 +1076,47 @@ template <int TM, int TN, int WM, int WN, int BK, int NST, bool SPLIT, int KIND>
         if (n > 0) cut += (long)n * ((kp + ch - 1) / ch);
     }
     // Cut only what is worth its traffic: four chunks or more, or fewer tiles than CUs (429 tiles of 832 columns in two chunks: 20 us,
-    // uncut 14 us)
-    a.cut = cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile && (tiles < CUS || cut >= 4l * (tiles - a.whole));
+    // uncut 14 us), and no tiles of 256 x 256
+    a.cut = TM <= 128 && cut <= COUNTERS && cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile && (tiles < CUS || cut >= 4l * (tiles - a.whole));
     hipLaunchKernelGGL((ns_gemm_kernel<TM, TN, WM, WN, BK, NST, SPLIT, KIND>), dim3((unsigned)(a.cut ? a.whole + cut : tiles)), dim3(TM / WM * (TN / WN) * 64), 0, st, a);
 }
 
-template <int TILE, bool SPLIT> int run_large(LargeArgs& a, hipStream_t st) {
+template <int TM, int TN, int KIND> long tiles_in(const Large& l) {
+    long n = 0;
+    for (int i = 0; i < l.count; ++i) n += (long)l.e[i].nsub * tiles_of<TM, TN, KIND>(l.e[i]);
+    return n;
+}
+
+// The tile of a product, by the number of tiles (us; f fp32 and SPLIT, b bf16 and single):
+//   A and B: 64 x 64 below 160 tiles of 128 x 128.  136 tiles (2048 x 2048), A: f 61 against 68, b 28 against 35; 113 of 12 matrices
+//   512 wide, B: f 21 against 34.  210 tiles (2560 x 2560), A: f 115 against 88, b 46 against 37.
+//   X: 256 x 256 (b, 8 waves) where rounds of 256 workgroups are 85 % full, never cut.  256 tiles: 156, in 128 x 128 183; 304 tiles:
+//   282 against 230; 36 tiles, cut: 143 against 30.  SPLIT 256 x 128: 112 against 114 at 256 tiles, 214 against 171 at 384: not used.
+//   64 x 64 does not pay: 144 tiles of 128 x 128 (1536 x 1536): f 45 against 61, b 30 against 28; 256 tiles: f 69 against 92, b 34 against 45.
+// Stages: two of 64 columns (four of 32, A b at 4096: 110 against 102); SPLIT two of 32 (three: 95 against 77).
+template <bool SPLIT, int KIND> void product_of_size(LargeArgs& a, hipStream_t st) {
+    constexpr int BK = SPLIT ? 32 : 64;
+    if (a.l.tile == 64) return product<64, 64, 32, 32, BK, 4, SPLIT, KIND>(a, st);
+    if constexpr (KIND == A_OF_X || KIND == B_OF_A) {
+        if (tiles_in<128, 128, KIND>(a.l) < 5 * CUS / 8) return product<64, 64, 32, 32, BK, 4, SPLIT, KIND>(a, st);
+    } else if constexpr (!SPLIT) {
+        const long wide = tiles_in<256, 256, KIND>(a.l);
+        if (20 * wide >= 17 * ((wide + CUS - 1) / CUS * CUS)) return product<256, 256, 128, 64, 32, 4, false, KIND>(a, st);
+    }
+    product<128, 128, 64, 64, BK, 2, SPLIT, KIND>(a, st);
+}
+
+template <bool SPLIT> int run_large(LargeArgs& a, hipStream_t st) {
     const int mode = mode_of(a.s);
     if (mode == F32) start_large<F32, SPLIT>(a, st);
     else if (mode == BF16) start_large<BF16, SPLIT>(a, st);
     else start_large<MUON, SPLIT>(a, st);
     KSR_LAUNCH_CHECK("muon_batch");
     for (a.k = 0; a.k < a.s.steps; ++a.k) {
-        const bool last = a.k + 1 == a.s.steps;
-        if constexpr (TILE == 64) {
-            constexpr int BK = SPLIT ? 32 : 64;
-            product<64, 64, 32, 32, BK, 4, SPLIT, A_OF_X>(a, st);
-            product<64, 64, 32, 32, BK, 4, SPLIT, B_OF_A>(a, st);
-            if (last) product<64, 64, 32, 32, BK, 4, SPLIT, X_LAST>(a, st);
-            else product<64, 64, 32, 32, BK, 4, SPLIT, X_NEXT>(a, st);
-        } else if constexpr (SPLIT) {
-            product<128, 128, 64, 64, 32, 2, true, A_OF_X>(a, st);
-            product<128, 128, 64, 64, 32, 2, true, B_OF_A>(a, st);
-            if (last) product<256, 128, 64, 64, 32, 3, true, X_LAST>(a, st);
-            else product<256, 128, 64, 64, 32, 3, true, X_NEXT>(a, st);
-        } else {
-            product<128, 128, 64, 64, 64, 2, false, A_OF_X>(a, st);
-            product<128, 128, 64, 64, 64, 2, false, B_OF_A>(a, st);
-            if (last) product<256, 256, 128, 64, 32, 4, false, X_LAST>(a, st);
-            else product<256, 256, 128, 64, 32, 4, false, X_NEXT>(a, st);
-        }
+        product_of_size<SPLIT, A_OF_X>(a, st);
+        product_of_size<SPLIT, B_OF_A>(a, st);
+        if (a.k + 1 < a.s.steps) product_of_size<SPLIT, X_NEXT>(a, st);
+        else product_of_size<SPLIT, X_LAST>(a, st);
         KSR_LAUNCH_CHECK("muon_batch");
     }
     return KSR_OK;
@@ -1182,8 +1207,7 @@ extern "C" int ksr_muon_batch(const KsrMatrix* mats, int count, int bf16, int sp
     for (int entry = 0, sub = 0; entry < count;) {
         if (!next_group(mats, count, split != 0, entry, sub, g.l, g.m)) break;
         int rc;
-        if (split) rc = g.l.tile == 128 ? run_large<128, true>(g, stream) : run_large<64, true>(g, stream);
-        else rc = g.l.tile == 128 ? run_large<128, false>(g, stream) : run_large<64, false>(g, stream);
+        rc = split ? run_large<true>(g, stream) : run_large<false>(g, stream);
         if (rc) return rc;
     }
     return KSR_OK;
