@@ -117,7 +117,7 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
     f32 = torch.float32
     if lr_dev is not None and (lr_dev.dtype is not f32 or lr_dev.numel() != 1 or lr_dev.device != device):
         raise KsrError("muon_update: lr_dev must be one float32 on the weights' device")
-    words, held, seen = [], [], set()
+    words, held, spans = [], [], []
     for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
         shape = as_matrix(w.shape)
         if shape is None:
@@ -136,11 +136,15 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
             g, rs, cs = g.contiguous(), cols, 1
             held.append(g)
         wp, mp = w.data_ptr(), m.data_ptr()
-        if wp and (wp in seen or mp in seen or wp == mp):
-            raise KsrError(f"muon_update: tensor {i}'s weight or momentum is in the list twice")
-        seen.add(wp)
-        seen.add(mp)
+        if wp:
+            nbytes = 4 * rows * cols
+            spans += (wp, wp + nbytes), (mp, mp + nbytes)
+            if g.data_ptr() in (wp, mp):
+                raise KsrError(f"muon_update: tensor {i}'s gradient is its weight or momentum")
         words += _matrix(g.data_ptr(), wp, mp, rs, cs, 0, rows, cols, 1)
+    spans.sort()
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):      # the matrices of a call run side by side
+        raise KsrError("muon_update: weights or momenta of the list overlap, or one is in it twice")
     _run(words, weights[0], False, _split(precision, f32), steps, coefficients, eps, True, momentum, nesterov, grad_scale, lr,
          lr_dev, weight_decay, scale)
     # the kernels write behind torch's back: whoever keys on the version counters (autograd, the UNet's kernel-layout weights) sees it

@@ -98,6 +98,19 @@ def test_wide_tiles(shape, dtype):
     compare(newton_schulz(u.cuda()), u, dtype is torch.float32)
 
 
+@pytest.mark.parametrize("shape,dtype", [((4, 1900, 1910), torch.bfloat16), ((4, 1910, 1900), torch.bfloat16),
+                                         ((3, 1400, 1500), torch.bfloat16), ((3, 1400, 1500), torch.float32),
+                                         ((3, 1500, 1400), torch.float32)])
+def test_widest_tiles(shape, dtype):
+    """Batches whose products take tiles of 128 for A and B, and the first two tiles of 256 for X with a last row and column of
+    tiles that are cut off."""
+    from kan_sr.muon import newton_schulz
+    u = gradients(shape, dtype, seed=8)
+    y = newton_schulz(u.cuda())
+    for k in (0, shape[0] - 1):
+        compare(y[k], u[k], dtype is torch.float32)
+
+
 @pytest.mark.parametrize("shape", [(48, 80), (200, 150)])
 def test_either_precision_for_either_type(shape):
     from kan_sr.muon import newton_schulz
@@ -236,6 +249,25 @@ def test_muon_update_of_a_list(nesterov):
             assert float((a.double().cpu() - w).norm()) <= (k + 1) * (1e-5 * step + 4 * 2.0 ** -24 * float(w.norm()))
 
 
+@pytest.mark.parametrize("precision,shapes", [("fp32", [(1400, 1500), (1500, 1400), (66, 4000)]),
+                                              ("bf16", [(1900, 1910), (1910, 1900), (1900, 1910), (1910, 1900)])])
+def test_muon_update_of_wide_matrices(precision, shapes):
+    from kan_sr.muon import muon_update
+    g = torch.Generator().manual_seed(26)
+    gs = [gradients(s, seed=30 + i) for i, s in enumerate(shapes)]
+    ws = [torch.randn(s, generator=g) * 0.1 for s in shapes]
+    W, M = [w.cuda() for w in ws], [torch.zeros(s, device="cuda") for s in shapes]
+    muon_update(W, [t.cuda() for t in gs], M, lr=0.02, weight_decay=0.1, precision=precision)
+    for k in (0, 1):
+        u = gs[k].double() * 1.95                      # of a zero momentum: m = g, U = g + 0.95 g
+        ref, rate = exact(u), 0.02 * 0.2 * max(shapes[k]) ** 0.5
+        # 8 x the model's error as in `compare`, and four roundings of the weight
+        tol = rate * (8 * (model(u, precision == "fp32") - ref).norm() + 32 * 2.0 ** -24 * ref.norm()) + 4 * 2.0 ** -24 * ws[k].norm()
+        err = W[k].double().cpu() - ((1 - 0.02 * 0.1) * ws[k].double() - rate * ref)
+        assert float(err.norm()) <= float(tol), (k, float(err.norm() / tol))
+        assert torch.equal(M[k].cpu(), gs[k])
+
+
 def test_gradient_layouts_learning_rate_on_the_device_and_repeats():
     from kan_sr.muon import muon_update
     g = torch.Generator().manual_seed(21)
@@ -309,6 +341,8 @@ def test_refusals_on_the_gpu():
            lambda: newton_schulz(w, eps=-1.0),
            lambda: muon_update([w], [w, w], [w], lr=0.1), lambda: muon_update([w[0]], [w[0]], [w[1]], lr=0.1),
            lambda: muon_update([w], [w.clone()], [w], lr=0.1), lambda: muon_update([w, w], [w, w], [w.clone(), w.clone()], lr=0.1),
+           lambda: muon_update([w], [w], [w.clone()], lr=0.1),
+           lambda: muon_update([w[:5], w[3:]], [w[:5].clone(), w[3:].clone()], [w[:5].clone(), w[3:].clone()], lr=0.1),
            lambda: muon_update([w.t()[:, :4]], [w[:, :4]], [w.clone()[:, :4].contiguous()], lr=0.1),
            lambda: muon_update([w], [w.bfloat16()], [w.clone()], lr=0.1), lambda: muon_update([w], [w[:4]], [w.clone()], lr=0.1),
            lambda: Muon([torch.nn.Parameter(w[0].clone())]), lambda: Muon([torch.nn.Parameter(w.clone())], lr=-1.0)]
