@@ -54,8 +54,7 @@ template <class V, bool PAST, class T> __device__ __forceinline__ void put(T* p,
 template <class T, int VEC> constexpr int in_flight() { return sizeof(T) * VEC == 16 ? 4 : 8; }
 
 // ------------------------------------------------------------------------------------------------ statistics
-// NE: entries (mean, M2) of a thread, each over VEC / NE channels of one group: 1 where a vector lies in one group, VEC / Cg where
-// it holds whole ones, VEC otherwise.
+// NE: entries (mean, M2) of a thread, each over the gcd(VEC, Cg) = VEC / NE neighbouring channels that always share a group
 template <class T, int VEC, int NE>
 __global__ void __launch_bounds__(THREADS) gn_stats_kernel(GnArgs a) {
     constexpr int PE = VEC / NE, R = in_flight<T, VEC>();
@@ -120,27 +119,34 @@ __global__ void __launch_bounds__(THREADS) gn_stats_kernel(GnArgs a) {
         }
     }
     __syncthreads();
-    // a wave per group that this channel block touches: join the entries of its channels and the pixel lanes
-    const int lane = threadIdx.x & 63, per = PE;
+    // L lanes per group that this channel block touches, all groups at once if they are few enough: join the entries of its
+    // channels and the pixel lanes
     const int g0 = w.c0 / a.Cg, g1 = (w.c0 + w.cb - 1) / a.Cg;
-    for (int g = g0 + ((int)threadIdx.x >> 6); g <= g1; g += THREADS / 64) {
-        const int lo = (g * a.Cg > w.c0 ? g * a.Cg - w.c0 : 0) / per;
-        const int hi = ((g + 1) * a.Cg < w.c0 + w.cb ? (g + 1) * a.Cg - w.c0 : w.cb) / per, ne = hi - lo;
+    int L = 64;
+    while (L > 4 && THREADS / L <= g1 - g0) L >>= 1;
+    const int lane = threadIdx.x & (L - 1);
+    auto sum_of = [&](float v) {
+        for (int m = L >> 1; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+        return v;
+    };
+    for (int g = g0 + (int)threadIdx.x / L; g <= g1; g += THREADS / L) {
+        const int lo = (g * a.Cg > w.c0 ? g * a.Cg - w.c0 : 0) / PE;
+        const int hi = ((g + 1) * a.Cg < w.c0 + w.cb ? (g + 1) * a.Cg - w.c0 : w.cb) / PE, ne = hi - lo;
         float cnt = 0.f, sum = 0.f;
-        for (int e = lane; e < a.PL * ne; e += 64) {
+        for (int e = lane; e < a.PL * ne; e += L) {
             const int pl = e / ne;
             cnt += sn[pl];
             sum = fmaf(sn[pl], smean[pl * a.CV * NE + lo + e - pl * ne], sum);
         }
-        cnt = wave_sum(cnt);
-        const float m = wave_sum(sum) / cnt;
+        cnt = sum_of(cnt);
+        const float m = sum_of(sum) / cnt;
         float q = 0.f;
-        for (int e = lane; e < a.PL * ne; e += 64) {
+        for (int e = lane; e < a.PL * ne; e += L) {
             const int pl = e / ne, k = pl * a.CV * NE + lo + e - pl * ne;
             const float d = smean[k] - m;
             q += fmaf(sn[pl] * d, d, sm2[k]);
         }
-        q = wave_sum(q);
+        q = sum_of(q);
         if (lane == 0) {
             float* o = a.part + 2 * (((w.b * a.nchunk + w.chunk) * a.nblk + w.blk) * a.GB + (g - g0));
             o[0] = m;
@@ -217,9 +223,11 @@ __device__ __forceinline__ void join_stats(const GnArgs& a, long b, float2* st, 
 template <int VEC> struct Affine {
     float mean[VEC], rstd[VEC], w[VEC], b[VEC];
     __device__ __forceinline__ Affine(const GnArgs& a, const float* stats, int c) {
+        int g = c / a.Cg, r = c - g * a.Cg;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float* s = stats + 2 * ((c + i) / a.Cg);
+            const float* s = stats + 2 * g;
+            if (++r == a.Cg) { r = 0; ++g; }
             mean[i] = s[0];
             rstd[i] = s[1];
             w[i] = a.w ? a.w[c + i] : 1.f;
@@ -473,9 +481,11 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_dx_kernel(GnArgs a) {
     const int c = w.c0 + w.tv * VEC;
     const Affine<VEC> k(a, a.stats + 2 * w.b * a.G, c);
     float q1[VEC], q2[VEC];
+    int g = c / a.Cg, r = c - g * a.Cg;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-        const float* s = coef + 2 * ((c + i) / a.Cg);
+        const float* s = coef + 2 * g;
+        if (++r == a.Cg) { r = 0; ++g; }
         q1[i] = s[0];
         q2[i] = s[1];
     }
@@ -507,12 +517,18 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_dx_kernel(GnArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// Number of workgroups that the chunks of a pass aim at: eight 256-thread workgroups on each of 256 CUs
-constexpr long AIM_WGS = 2048;
+// Number of workgroups that the chunks of a pass aim at: eight 256-thread workgroups on each of 256 CUs; fewer, down to two, where
+// a workgroup would have less than MIN_TILES turns of its loop, whose start and join then cost more than its work
+// (2 x 128 x 128 x 320 bf16, one turn: statistics and result 10.2 + 17.4 us; three: 8.9 + 12.4 us).
+constexpr long AIM_WGS = 2048, LEAST_WGS = 512, MIN_TILES = 8;
+// Chunks that the pass which uses their results joins itself, rather than a launch in between: as many values a workgroup reads
+constexpr long JOIN_VALUES = 4096;
 constexpr int64_t PAST_BYTES = 64 << 20;            // results of a quarter of the last-level cache or more are written past it
 
-// Split of [B, S, C] for a vector of `vec` channels, `inflight` pixels a thread holds at once
-void split(GnArgs& a, int vec, int inflight) {
+// Split of [B, S, C] for a vector of `vec` channels, `inflight` pixels a thread holds at once.  A chunk has G (forward) or C
+// (backward) results; half as many chunks as would fit are taken if they can be joined without a launch (one channel block, at
+// most THREADS results) and each CU still has a workgroup (the case above: one launch of 6 us less, 1 us more in each pass).
+void split(GnArgs& a, int vec, int inflight, bool backward) {
     const int vectors = a.C / vec;
     a.nblk = (vectors + THREADS - 1) / THREADS;
     a.CV = (vectors + a.nblk - 1) / a.nblk;
@@ -523,10 +539,17 @@ void split(GnArgs& a, int vec, int inflight) {
     if (a.GB > a.G) a.GB = a.G;
     const long tile = (long)a.PL * inflight, tiles = (a.S + tile - 1) / tile;
     long want = AIM_WGS / (a.B * a.nblk > AIM_WGS ? AIM_WGS : a.B * a.nblk);
+    const long few = tiles / MIN_TILES, least = LEAST_WGS / (a.B * a.nblk);
+    if (want > few) want = few > least ? few : least;
+    const int results = backward ? a.C : a.G;
+    const long joined = JOIN_VALUES / results;
+    const bool joins = a.nblk == 1 && results <= THREADS;
+    if (joins && want > joined && want <= 2 * joined && 2 * joined * a.B >= LEAST_WGS) want = joined;
     if (want < 1) want = 1;
     if (want > tiles) want = tiles;
     a.chunk = (tiles + want - 1) / want * tile;
     a.nchunk = (a.S + a.chunk - 1) / a.chunk;
+    a.join = joins && a.nchunk * results <= JOIN_VALUES;
 }
 
 // most chunks that split() makes for any vector width
@@ -537,7 +560,7 @@ long max_parts(long B, long S, int C, int G, bool backward) {
             if (C % vec) continue;
             GnArgs a{};
             a.B = B; a.S = S; a.C = C; a.G = G; a.Cg = C / G;
-            split(a, vec, fl);
+            split(a, vec, fl, backward);
             const long n = B * a.nchunk * 2 * (backward ? C : (long)a.nblk * a.GB);
             if (n > most) most = n;
         }
@@ -559,9 +582,11 @@ int vec_of(const GnArgs& a, int esize, bool backward) {
 
 template <class T, int VEC> void stats(const GnArgs& a, dim3 grid, hipStream_t st) {
     const dim3 block(THREADS);
-    if (a.Cg % VEC == 0) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, 1>), grid, block, 0, st, a);
-    else if (VEC > 2 && VEC % a.Cg == 0 && VEC / a.Cg == 2) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, (VEC > 2 ? 2 : 1)>), grid, block, 0, st, a);
-    else if (VEC > 4 && VEC % a.Cg == 0 && VEC / a.Cg == 4) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, (VEC > 4 ? 4 : 1)>), grid, block, 0, st, a);
+    int per = VEC;                                      // gcd(VEC, Cg): VEC is a power of two
+    while (a.Cg % per) per >>= 1;
+    if (per == VEC) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, 1>), grid, block, 0, st, a);
+    else if (VEC > 2 && 2 * per == VEC) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, (VEC > 2 ? 2 : 1)>), grid, block, 0, st, a);
+    else if (VEC > 4 && 4 * per == VEC) hipLaunchKernelGGL((gn_stats_kernel<T, VEC, (VEC > 4 ? 4 : 1)>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((gn_stats_kernel<T, VEC, VEC>), grid, block, 0, st, a);
 }
 
@@ -571,10 +596,8 @@ template <class T, int VEC, int ACT> void apply(const GnArgs& a, dim3 grid, hipS
 }
 
 template <class T, int VEC> int run_fwd(GnArgs& a, int act, hipStream_t st) {
-    split(a, VEC, in_flight<T, VEC>());
+    split(a, VEC, in_flight<T, VEC>(), false);
     const dim3 grid((unsigned)(a.B * a.nblk * a.nchunk)), block(THREADS);
-    // the statistics are joined by every workgroup that uses them where that is at most 128 values for a lane pair to read
-    a.join = a.nblk == 1 && a.G <= THREADS && a.nchunk * a.G <= 4096;
     stats<T, VEC>(a, grid, st);
     KSR_LAUNCH_CHECK("group_norm_fwd");
     if (!a.join) {
@@ -592,10 +615,9 @@ template <class T, int VEC> int run_fwd(GnArgs& a, int act, hipStream_t st) {
 }
 
 template <class T, int VEC, int ACT> int run_bwd_act(GnArgs& a, hipStream_t st) {
-    split(a, VEC, in_flight<T, VEC>() / 2);
+    split(a, VEC, in_flight<T, VEC>() / 2, true);
     const dim3 block(THREADS);
     const long work = a.B * a.nblk * a.nchunk;
-    a.join = a.nblk == 1 && a.C <= THREADS && a.nchunk * a.C <= 4096;
     hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, VEC, ACT>), dim3((unsigned)work), block, 0, st, a);
     KSR_LAUNCH_CHECK("group_norm_bwd");
     if (!a.join) {
