@@ -44,7 +44,7 @@ template <int VEC> struct Place {
 
 template <class V, class T> __device__ __forceinline__ typename V::Raw ld(const T* p) { return *reinterpret_cast<const typename V::Raw*>(p); }
 // Results past the caches where they are large: the pass that writes them reads x (and dy) a second time, and what of it the
-// caches still hold stays there (4 x 512 x 512 x 128 bf16: 161 instead of 180 us).  Smaller results are left to whoever reads next.
+// caches still hold stays there (4 x 512 x 512 x 128 bf16: 155 instead of 174 us).  Smaller results are left to whoever reads next.
 template <class V, bool PAST, class T> __device__ __forceinline__ void put(T* p, const typename V::Raw& v) {
     if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<typename V::Raw*>(p));
     else *reinterpret_cast<typename V::Raw*>(p) = v;

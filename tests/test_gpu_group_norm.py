@@ -105,6 +105,18 @@ def test_values_and_gradients(shape, G, dtype):
     check(*case(shape, G, dtype, act), G, act)
 
 
+# too large for one workgroup: groups of 12, 10, 6, 7 and 1 channels (vectors share 4, 2, 1 of them), of several channel blocks, of
+# more chunks than are joined without a launch
+CHUNKED = [((1, 48, 50, 24), 2), ((2, 47, 47, 40), 4), ((1, 3000, 24), 4), ((1, 2500, 56), 8), ((1, 16500, 136), 136),
+           ((1, 400, 2080), 5), ((2, 130, 127, 320), 32)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,G", CHUNKED)
+def test_groups_in_chunks(shape, G, dtype):
+    check(*case(shape, G, dtype, "silu", seed=9), G, "silu")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
 def test_every_activation(act, dtype):
