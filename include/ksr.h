@@ -579,7 +579,8 @@ int ksr_adam_step_dev(float* params, const float* grads, float* exp_avg, float* 
                       const float* lr_dev, float beta1, float beta2, float eps, float weight_decay,
                       const uint64_t* step_dev, float grad_scale, ksr_stream_t stream);
 
-/* Either form over parts of the flat buffers: runs is a HOST array of n_runs (first, length) pairs.  lr_dev and step_dev
+/* Either form over parts of the flat buffers: runs is a HOST array of n_runs (first, length) pairs in ascending order that do
+ * not overlap.  lr_dev and step_dev
  * (both or neither) replace lr and step as in ksr_adam_step_dev.  The rest of the buffers is not touched (the parameters that
  * ksr_muon_batch updates). */
 int ksr_adam_step_runs(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, const int64_t* runs, int n_runs,
@@ -794,7 +795,7 @@ int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t x_pixel_st
  * split != 0: products of f16 pairs (22 bits), as close to 64 bits as fp32 arithmetic; 0: single f16 operands (diagonals and
  *   the linear term apart), about 1e-3 off, for bf16 results.
  * mats: HOST array, read during the call.  src may have any non-negative element strides; src and dst may be the same memory.
- * The matrices of one call must not overlap in dst and momentum.  lr_dev: NULL, or a device float that replaces lr (recorded
+ * Nothing that one matrix of a call writes (dst, momentum) may overlap what another reads or writes.  lr_dev: NULL, or a device float that replaces lr (recorded
  * graphs).  ws: ksr_muon_ws_bytes bytes of device memory, 16-byte aligned, free again when the call's kernels have run; calls
  * that may overlap need one each.  A matrix with a non-finite element becomes NaN throughout.  Refused: coefficients with
  * which a singular value, or an eigenvalue of A or b A + c A A, could pass 30 within the steps. */

@@ -235,9 +235,13 @@ extern "C" int ksr_adam_step_runs(float* params, const float* grads, float* exp_
                                   const uint64_t* step_dev, float grad_scale, hipStream_t stream) {
     KSR_CHECK_ARG(params && grads && exp_avg && exp_avg_sq && (runs || n_runs == 0) && n_runs >= 0, "adam_step_runs: bad argument");
     KSR_CHECK_ARG((lr_dev != nullptr) == (step_dev != nullptr) && (step_dev || step >= 1), "adam_step_runs: a step count from 1, or lr_dev and step_dev");
-    for (int i = 0; i < n_runs; ++i)
-        KSR_CHECK_ARG(runs[2 * i] >= 0 && runs[2 * i + 1] >= 0 && runs[2 * i + 1] < (1ll << 31), "adam_step_runs: run %d is (%lld, %lld)", i,
-                      (long long)runs[2 * i], (long long)runs[2 * i + 1]);
+    int64_t end = 0;                                    // of the run before: no element may be updated twice
+    for (int i = 0; i < n_runs; ++i) {
+        KSR_CHECK_ARG(runs[2 * i] >= end && runs[2 * i + 1] >= 0 && runs[2 * i + 1] < (1ll << 31),
+                      "adam_step_runs: run %d is (%lld, %lld), the one before ends at %lld", i, (long long)runs[2 * i],
+                      (long long)runs[2 * i + 1], (long long)end);
+        end = runs[2 * i] + runs[2 * i + 1];
+    }
     const float bc1 = (float)(1.0 - pow((double)beta1, (double)step));
     const float bc2_sqrt = (float)sqrt(1.0 - pow((double)beta2, (double)step));
     for (int base = 0; base < n_runs; base += ADAM_RUNS) {

@@ -120,6 +120,7 @@ def test_adam_runs_refusals():
     assert call(None, 1) == -1 and call(two, -1) == -1 and call(two, 1, step=0) == -1 and call(two, 1, lr_dev=fake) == -1
     assert call((c_int64 * 2)(-1, 4), 1) == -1 and call((c_int64 * 2)(0, 1 << 31), 1) == -1
     assert call(two, 0) == 0 and call((c_int64 * 2)(0, 0), 1) == 0
+    assert call((c_int64 * 4)(0, 4, 3, 2), 2) == -1 and call((c_int64 * 4)(4, 2, 0, 2), 2) == -1 and call((c_int64 * 4)(7, 0, 7, 0), 2) == 0
 
 
 def test_group_norm_unet_has_the_batch_norm_keys_without_running_statistics():
