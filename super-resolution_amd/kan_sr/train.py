@@ -396,6 +396,8 @@ class TrainStep:
         """This step's _body through the HIP graph of the current input shape (recorded on the third step at that
         shape; the two before it run unrecorded and size every lazily allocated workspace)."""
         key = (tuple(x.shape), tuple(tgt.shape), self.model.training, self.model.precision)
+        if self._adam_in_body():                # what the recorded optimiser launches hold by value: a change records anew
+            key += (tuple(self.betas), self.eps, self.wd, self.muon_momentum)
         ent = self._graphs.get(key)
         if ent is None:
             ent = self._graphs[key] = dict(graph=None, warm=0, gx=torch.empty_like(x),

@@ -210,6 +210,23 @@ def test_captured_muon_step_equals_launched_step(backbone):
     assert runs[0][0] == runs[1][0] and torch.equal(runs[0][1], runs[1][1]) and torch.equal(runs[0][2], runs[1][2])
 
 
+def test_changed_momentum_is_not_replayed_from_an_old_graph():
+    from kan_sr.module import ConvSepKan
+    from kan_sr.train import TrainStep
+    runs = []
+    for capture in (False, True):
+        torch.manual_seed(34)
+        m = ConvSepKan([1], [4], [3], 5, 3, 0.1, [-1, 1], 2).eval().cuda()
+        ts = TrainStep(m, lr=1e-3, optimizer="muon", capture=capture, device_state=True)
+        gen = torch.Generator().manual_seed(8)
+        for it in range(8):
+            if it == 4:
+                ts.muon_momentum, ts.betas = 0.5, (0.8, 0.99)
+            ts.step(torch.rand(2, 3, 32, 32, generator=gen).cuda(), torch.rand(2, 3, 64, 64, generator=gen).cuda())
+        runs.append((ts.flat_p.clone(), ts.exp_avg.clone()))
+    assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1])
+
+
 def test_muon_checkpoint_resumes_and_does_not_mix_with_adam(tmp_path):
     from kan_sr._lib import KsrError
     from kan_sr.checkpoint import load_checkpoint, save_checkpoint
