@@ -49,7 +49,8 @@ __device__ __forceinline__ float clamp01(float v) { return fminf(fmaxf(v, 0.f), 
 // 512 x 512, 266 us) the vertical filter accounts for 76 us, the horizontal one for 90, the evaluation of S for 47 and
 // loads / LDS / barriers for the rest, the parts adding up; a variant with three waves per SIMD instead of two (runs of 5
 // windows, 6-row sub-batches: 168 registers, 17 KB of LDS) ran in the same time.  About 5 cycles per vector instruction and
-// SIMD (two thirds of them packed) is what this chip sustains on such a stream.
+// SIMD (two thirds of them packed) is what this chip sustained on such a stream; the build has no packed fp32 instructions any
+// more (64 x 3 x 512 x 512: 250 us with them, 306 us without).
 constexpr int SV_T = 128;                       // two waves: four workgroups give every SIMD of a CU its two waves (three-wave
                                                 // workgroups left two of the four SIMDs with one)
 constexpr int SV_WO = SV_T - (SS_K - 1);        // window columns per strip at most
