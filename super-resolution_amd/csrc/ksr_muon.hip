@@ -624,7 +624,7 @@ template <int TM, int TN, int WM, int WN, int BK, int NST, bool SPLIT, int KIND>
 __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) == 4 ? 2 : 1) ns_gemm_kernel(LargeArgs a) {
     constexpr int WC = TN / WN, WAVES = TM / WM * WC, TH = 64 * WAVES;
     constexpr int NP = SPLIT ? 2 : 1, MT = WM / 32, NT = WN / 32, CH = BK / 8;
-    constexpr bool ODD = TM > 128 || TN > 128;                          // buffers are padded to 128: the last tile may be cut off
+    constexpr bool WIDE = TM > 128 || TN > 128;                          // buffers are padded to 128: the last tile may be cut off
     constexpr int PBYTES = TM * BK * 2, QBYTES = TN * BK * 2, STAGE = NP * (PBYTES + QBYTES);
     constexpr int HALVES = NST * STAGE >= TM * (TN + 8) * 2 && NST * STAGE >= TN * (TM + 8) * 2 ? 1 : 2;      // the output tile reuses the stages
     static_assert(NST * STAGE >= TM / HALVES * (TN + 8) * 2 && NST * STAGE >= TN * (TM / HALVES + 8) * 2 && TM / HALVES >= WM, "output tile");
@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
 #pragma unroll
             for (int i = 0; i < PI; ++i) {
                 const int row = (wave * PI + i) * ROWS + drow;
-                const _Float16* src = P + pl * pp + place(pr, !ODD || row < rows ? row : 0, kt * BK + 8 * (dslot ^ f(row)));
+                const _Float16* src = P + pl * pp + place(pr, !WIDE || row < rows ? row : 0, kt * BK + 8 * (dslot ^ f(row)));
                 ksr_dma16<false>(src, to + pl * PBYTES + (wave * PI + i) * 1024);
             }
 #pragma unroll
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
         for (int x = 0; x < MT; ++x)
 #pragma unroll
             for (int y = 0; y < NT; ++y) acc[x][y] = sum[x][y];
-    if (slices > 1) {
+    if (!WIDE && slices > 1) {
         int* counter = reinterpret_cast<int*>(a.l.ws + a.l.o_part) + slot;
         float* part = reinterpret_cast<float*>(a.l.ws + a.l.o_part + 4l * COUNTERS) + (long)slot * TM * TN + threadIdx.x;
         float* own = part + (long)slice * TM * TN;
@@ -852,7 +852,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                         v[z] *= S;
                     }
                 } else if constexpr (KIND == B_OF_A) {
-                    if (ODD && row0 - ti * TM >= rows) continue;
+                    if (WIDE && row0 - ti * TM >= rows) continue;
                     const h4 rh = *reinterpret_cast<const h4*>(R + place(l.mp, c, row0));       // R is symmetric
                     h4 rl = {};
                     if constexpr (SPLIT) rl = *reinterpret_cast<const h4*>(R + pp + place(l.mp, c, row0));
@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                             v[z] = 0.f;
                         } else v[z] = S * (sp.b * r + sp.c * ((di + dc) * r + sq));
                     }
-                } else if (!ODD || (row0 - ti * TM < rows && c - tj * TN < cols)) {
+                } else if (!WIDE || (row0 - ti * TM < rows && c - tj * TN < cols)) {
                     const float alpha = xi * INV_S;
                     const long plane = (long)l.mp * l.np;
                     if (!swap) {                        // rows are i, columns j
@@ -898,7 +898,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                 }
 #pragma unroll
                 for (int z = 0; z < 4; ++z) acc[x][y][4 * g + z] = v[z];
-                if (ODD && g == 3) __builtin_amdgcn_sched_barrier(0);        // more of X^T in flight would spill
+                if (WIDE && g == 3) __builtin_amdgcn_sched_barrier(0);        // more of X^T in flight would spill
             }
         }
     if constexpr (KIND == X_LAST) return;
@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
 #pragma unroll
             for (int half = 0; half < HALVES; ++half) {
                 constexpr int HM = TM / HALVES;                      // rows of the tile in LDS at a time
-                if constexpr (ODD)                                       // nothing rounded is kept for the next round: it would spill
+                if constexpr (WIDE)                                       // nothing rounded is kept for the next round: it would spill
 #pragma unroll
                     for (int x = 0; x < MT; ++x)
 #pragma unroll
@@ -959,7 +959,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                     const int i = tr ? c : r, j = tr ? r : c;        // row and column of the product's tile
                     // what lies beyond an odd number of 128s is not stored; of a symmetric product, nothing above the diagonal's
                     // blocks of TN, and the transposes of those below it
-                    bool ok = !ODD || (half * HM + i < rows && j < cols);
+                    bool ok = !WIDE || (half * HM + i < rows && j < cols);
                     if constexpr (SYM) {
                         const int bi = (i0 + i) / TN;
                         ok = ok && (tr ? bi > tj : bi >= tj);
@@ -1078,7 +1078,7 @@ template <int TM, int TN, int WM, int WN, int BK, int NST, bool SPLIT, int KIND>
     }
     // Cut only what is worth its traffic: four chunks or more, or fewer tiles than CUs (429 tiles of 832 columns in two chunks: 20 us,
     // uncut 14 us), and no tiles of 256 x 256
-    a.cut = TM <= 128 && cut <= COUNTERS && cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile && (tiles < CUS || cut >= 4l * (tiles - a.whole));
+    a.cut = TM * TN <= 128 * 128 && cut <= COUNTERS && cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile && (tiles < CUS || cut >= 4l * (tiles - a.whole));
     hipLaunchKernelGGL((ns_gemm_kernel<TM, TN, WM, WN, BK, NST, SPLIT, KIND>), dim3((unsigned)(a.cut ? a.whole + cut : tiles)), dim3(TM / WM * (TN / WN) * 64), 0, st, a);
 }
 
@@ -1094,12 +1094,13 @@ template <int TM, int TN, int KIND> long tiles_in(const Large& l) {
 //   X: 256 x 256 (b, 8 waves) where rounds of 256 workgroups are 85 % full, never cut.  256 tiles: 156, in 128 x 128 183; 304 tiles:
 //   282 against 230; 36 tiles, cut: 143 against 30.  SPLIT 256 x 128: 112 against 114 at 256 tiles, 214 against 171 at 384: not used.
 //   64 x 64 does not pay: 144 tiles of 128 x 128 (1536 x 1536): f 45 against 61, b 30 against 28; 256 tiles: f 69 against 92, b 34 against 45.
-// Stages: two of 64 columns (four of 32, A b at 4096: 110 against 102); SPLIT two of 32 (three: 95 against 77).
+// Stages: two of 64 columns (four of 32, A b at 4096: 110 against 102); SPLIT two of 32 (three: 95 against 77).  64 x 64: three, so
+// that three workgroups share a CU (four: A at 1024 x 4096 f 45 against 39, b 27 against 23; two: 777 x 2051 b 255 against 245).
 template <bool SPLIT, int KIND> void product_of_size(LargeArgs& a, hipStream_t st) {
     constexpr int BK = SPLIT ? 32 : 64;
-    if (a.l.tile == 64) return product<64, 64, 32, 32, BK, 4, SPLIT, KIND>(a, st);
+    if (a.l.tile == 64) return product<64, 64, 32, 32, BK, 3, SPLIT, KIND>(a, st);
     if constexpr (KIND == A_OF_X || KIND == B_OF_A) {
-        if (tiles_in<128, 128, KIND>(a.l) < 5 * CUS / 8) return product<64, 64, 32, 32, BK, 4, SPLIT, KIND>(a, st);
+        if (tiles_in<128, 128, KIND>(a.l) < 5 * CUS / 8) return product<64, 64, 32, 32, BK, 3, SPLIT, KIND>(a, st);
     } else if constexpr (!SPLIT) {
         const long wide = tiles_in<256, 256, KIND>(a.l);
         if (20 * wide >= 17 * ((wide + CUS - 1) / CUS * CUS)) return product<256, 256, 128, 64, 32, 4, false, KIND>(a, st);
