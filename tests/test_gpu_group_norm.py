@@ -222,6 +222,31 @@ def test_side_stream_and_repeated_runs_are_bit_equal():
     assert all(torch.equal(a, c) for a, c in zip(first, second))
 
 
+def test_calls_on_two_streams_at_once():
+    from kan_sr.ops import group_norm_act
+    cases = [case(s, G, t, "silu", seed=11) + (G,) for s, G, t in
+             (((2, 130, 127, 320), 32, torch.bfloat16), ((4, 64, 64, 64), 8, torch.float32), ((1, 90, 90, 24), 2, torch.float32))]
+
+    def run(x, w, b, dy, G):
+        x, w, b = (t.cuda().requires_grad_() for t in (x, w, b))
+        dy = dy.cuda()
+        torch.cuda.current_stream().synchronize()
+        y = group_norm_act(x, G, w, b, activation="silu")
+        return (y,) + torch.autograd.grad(y, (x, w, b), dy)
+
+    want = [run(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for k in range(3):
+        for c, st in zip(cases, streams):
+            with torch.cuda.stream(st):
+                got.append(run(*c))
+    torch.cuda.synchronize()
+    for k, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[k % 3])), k
+
+
 def test_captured_into_a_graph_and_replayed():
     from kan_sr.ops import group_norm_act
     x, w, b, dy = (t.cuda() for t in case((2, 31, 30, 40), 4, torch.float32, "silu", seed=13))

@@ -214,6 +214,38 @@ def test_large_batches_run_in_parts():
     compare(y[:2].contiguous(), u[:2], True)
 
 
+def test_calls_on_two_streams_at_once():
+    from kan_sr.muon import newton_schulz
+    us = [gradients((900, 1000), seed=40).cuda(), gradients((2, 300, 2500), torch.bfloat16, seed=41).cuda(), gradients((20, 64, 900), seed=42).cuda()]
+    want = [newton_schulz(u) for u in us]
+    streams = [torch.cuda.Stream() for _ in us]
+    torch.cuda.synchronize()
+    got = []
+    for k in range(4):
+        for u, st in zip(us, streams):
+            with torch.cuda.stream(st):
+                got.append(newton_schulz(u))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[k % 3]) for k, y in enumerate(got))
+
+
+@pytest.mark.parametrize("rows", [40, 80])
+def test_offsets_beyond_32_bits(rows):
+    """Rows, then matrices, so far apart that the last one lies more than 2^31 elements (and 2^32 bytes) behind the first."""
+    from kan_sr.muon import newton_schulz
+    u = gradients((rows, 100), torch.bfloat16, seed=43)
+    want = newton_schulz(u.cuda())
+    step = (1 << 31) // (rows - 1) + 8
+    big = torch.empty((rows - 1) * step + 100, dtype=torch.bfloat16, device="cuda")
+    far = big.as_strided((rows, 100), (step, 1))
+    far.copy_(u)
+    assert torch.equal(newton_schulz(far), want)
+    two = big.as_strided((2, rows, 100), ((rows - 1) * step - rows * 100, 100, 1))
+    two.copy_(u.expand(2, rows, 100))
+    y = newton_schulz(two)
+    assert torch.equal(y[0], y[1]) and torch.equal(y, newton_schulz(u.cuda().expand(2, rows, 100)))
+
+
 # ------------------------------------------------------------------------------------------------ the Muon update
 LIST = [(192, 64), (64, 64), (32, 64), (64, 32), (64, 64, 1, 1), (160, 64, 1, 1), (8, 4, 3, 3), (70, 200), (200, 70), (70, 200), (64, 1, 3, 3)]
 
@@ -266,6 +298,22 @@ def test_muon_update_of_wide_matrices(precision, shapes):
         err = W[k].double().cpu() - ((1 - 0.02 * 0.1) * ws[k].double() - rate * ref)
         assert float(err.norm()) <= float(tol), (k, float(err.norm() / tol))
         assert torch.equal(M[k].cpu(), gs[k])
+
+
+def test_long_lists_are_updated_like_their_entries():
+    """More entries than a launch takes: 50 small and 30 large matrices of different shapes, mixed."""
+    from kan_sr.muon import muon_update
+    g = torch.Generator().manual_seed(27)
+    shapes = [(8 + i, 40 + 7 * i) for i in range(50)] + [(66 + 3 * i, 150 - 2 * i) for i in range(30)]
+    shapes = [shapes[(37 * i) % 80] for i in range(80)]
+    w0 = [torch.randn(s, generator=g).cuda() for s in shapes]
+    gs = [1e-3 * torch.randn(s, generator=g).cuda() for s in shapes]
+    W, M = [t.clone() for t in w0], [torch.zeros_like(t) for t in w0]
+    muon_update(W, gs, M, lr=0.02, weight_decay=0.1)
+    for w, grad, a, b in zip(w0, gs, W, M):
+        m = torch.zeros_like(w)
+        muon_update([w], [grad], [m], lr=0.02, weight_decay=0.1)
+        assert torch.equal(w, a) and torch.equal(m, b), tuple(w.shape)
 
 
 def test_gradient_layouts_learning_rate_on_the_device_and_repeats():
