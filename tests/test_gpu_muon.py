@@ -123,6 +123,21 @@ def test_either_precision_for_either_type(shape):
     compare(newton_schulz(u.bfloat16().cuda(), precision="fp32"), u.bfloat16(), True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(90, 30), (1000, 63), (1000, 62), (500, 60), (3, 70, 12), (900, 4)])
+def test_tall_small_matrices(shape, dtype):
+    """Rows that are, and are not, whole groups of four values; the same values behind an address that is not a multiple."""
+    from kan_sr.muon import newton_schulz
+    u = gradients(shape, dtype, seed=44)
+    y = newton_schulz(u.cuda())
+    compare(y, u, True)
+    wide = torch.zeros(*shape[:-1], shape[-1] + 5, dtype=dtype, device="cuda")
+    for lo in (1, 4):
+        part = wide[..., lo:lo + shape[-1]]
+        part.copy_(u)
+        assert torch.equal(newton_schulz(part), y)
+
+
 def test_strides_are_read_in_place():
     from kan_sr.muon import newton_schulz
     for m, n in ((40, 100), (150, 210)):
@@ -298,6 +313,30 @@ def test_muon_update_of_wide_matrices(precision, shapes):
         err = W[k].double().cpu() - ((1 - 0.02 * 0.1) * ws[k].double() - rate * ref)
         assert float(err.norm()) <= float(tol), (k, float(err.norm() / tol))
         assert torch.equal(M[k].cpu(), gs[k])
+
+
+@pytest.mark.parametrize("lo", [1, 2, 4])
+def test_parts_of_a_flat_buffer_at_any_offset(lo):
+    from kan_sr.muon import muon_update
+    g = torch.Generator().manual_seed(28)
+    shapes = [(192, 64), (64, 192), (90, 30), (200, 72), (72, 200), (100, 99)]
+    src = [[torch.randn(s, generator=g).cuda() for s in shapes] for _ in range(2)]
+    grads = [1e-3 * torch.randn(s, generator=g).cuda() for s in shapes]
+    W, M = ([t.clone() for t in part] for part in src)
+    muon_update(W, grads, M, lr=0.02)
+    flats = []
+    for part in src + [grads]:
+        flat, views, off = torch.zeros(lo + sum(t.numel() + 3 for t in part), device="cuda"), [], lo
+        for t in part:
+            views.append(flat[off:off + t.numel()].view(t.shape).copy_(t))
+            off += t.numel() + 3
+        flats.append((flat, views))
+    muon_update(flats[0][1], flats[2][1], flats[1][1], lr=0.02)
+    assert all(torch.equal(a, b) for a, b in zip(flats[0][1] + flats[1][1], W + M))
+    for flat, views in flats[:2]:                      # what lies between the parts is left as it was
+        for v in views:
+            v.zero_()
+        assert not bool(flat.any())
 
 
 def test_long_lists_are_updated_like_their_entries():
