@@ -1101,8 +1101,8 @@ bool bounded(float a, float b, float c, int steps, float& log2_gain) {
     double top = 1.0, g = fabs((double)a);
     for (int k = 0; k < steps; ++k) {
         double next = 0;
-        for (int i = 0; i <= 512; ++i) {
-            const double s = top * 1.02 * i / 512, s2 = s * s, f = a + b * s2 + c * s2 * s2;
+        for (int i = 0; i <= 128; ++i) {
+            const double s = top * 1.02 * i / 128, s2 = s * s, f = a + b * s2 + c * s2 * s2;
             if (fabs(f) > g) g = fabs(f);
             if (fabs(f) * s > next) next = fabs(f) * s;
             if (!(s2 <= 30) || !(fabs(b * s2 + c * s2 * s2) <= 30) || !(fabs(f) * s <= 30)) return false;

@@ -117,34 +117,40 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
     f32 = torch.float32
     if lr_dev is not None and (lr_dev.dtype is not f32 or lr_dev.numel() != 1 or lr_dev.device != device):
         raise KsrError("muon_update: lr_dev must be one float32 on the weights' device")
+    every = weights + grads + momenta
+    if {t.dtype for t in every} != {f32} or {t.get_device() for t in every} != {device.index}:
+        raise KsrError(f"muon_update: every weight, gradient and momentum must be float32 on {device}")
     words, held, spans = [], [], []
     for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
-        shape = as_matrix(w.shape)
-        if shape is None:
-            raise KsrError(f"muon_update: tensor {i} is {tuple(w.shape)}: matrices only (vectors belong to Adam)")
-        rows, cols = shape
-        if rows > 1 << 24 or cols > 1 << 24:
-            raise KsrError(f"muon_update: tensor {i}: {tuple(w.shape)} is too large")
-        if not (w.dtype is g.dtype is m.dtype is f32) or w.device != device or g.device != device or m.device != device:
-            raise KsrError(f"muon_update: tensor {i}: weight, gradient and momentum must be float32 on {device}")
-        if g.shape != w.shape or m.shape != w.shape or not w.is_contiguous() or not m.is_contiguous():
-            raise KsrError(f"muon_update: tensor {i}: gradient and momentum must have the weight's shape {tuple(w.shape)}, weight "
+        shape = w.shape
+        if len(shape) < 2:
+            raise KsrError(f"muon_update: tensor {i} is {tuple(shape)}: matrices only (vectors belong to Adam)")
+        if g.shape != shape or m.shape != shape or not w.is_contiguous() or not m.is_contiguous():
+            raise KsrError(f"muon_update: tensor {i}: gradient and momentum must have the weight's shape {tuple(shape)}, weight "
                            "and momentum be contiguous")
-        if g.dim() == 2:
+        if len(shape) == 2:
+            rows, cols = shape
             rs, cs = g.stride()
         else:
+            rows, cols = as_matrix(shape)
             g, rs, cs = g.contiguous(), cols, 1
             held.append(g)
-        wp, mp = w.data_ptr(), m.data_ptr()
+        if rows > 1 << 24 or cols > 1 << 24:
+            raise KsrError(f"muon_update: tensor {i}: {tuple(shape)} is too large")
+        wp, gp, mp = w.data_ptr(), g.data_ptr(), m.data_ptr()
         if wp:
             nbytes = 4 * rows * cols
-            spans += (wp, wp + nbytes), (mp, mp + nbytes)
-            if g.data_ptr() in (wp, mp):
+            spans.append((wp, wp + nbytes))
+            spans.append((mp, mp + nbytes))
+            if gp == wp or gp == mp:
                 raise KsrError(f"muon_update: tensor {i}'s gradient is its weight or momentum")
-        words += _matrix(g.data_ptr(), wp, mp, rs, cs, 0, rows, cols, 1)
+        words += gp, wp, mp, rs, cs, 0, rows | cols << 32, 1                # _matrix(...)
     spans.sort()
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):      # the matrices of a call run side by side
-        raise KsrError("muon_update: weights or momenta of the list overlap, or one is in it twice")
+    end = 0
+    for first, last in spans:                                   # the matrices of a call run side by side
+        if first < end:
+            raise KsrError("muon_update: weights or momenta of the list overlap, or one is in it twice")
+        end = last
     _run(words, weights[0], False, _split(precision, f32), steps, coefficients, eps, True, momentum, nesterov, grad_scale, lr,
          lr_dev, weight_decay, scale)
     # the kernels write behind torch's back: whoever keys on the version counters (autograd, the UNet's kernel-layout weights) sees it
@@ -178,14 +184,15 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             weights, grads, momenta = [], [], []
             for p in group["params"]:
-                if p.grad is None:
+                g = p.grad
+                if g is None:
                     continue
-                state = self.state[p]
-                if "momentum_buffer" not in state:
-                    state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                m = self.state[p].get("momentum_buffer")
+                if m is None:
+                    m = self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                 weights.append(p)
-                grads.append(p.grad)
-                momenta.append(state["momentum_buffer"])
+                grads.append(g)
+                momenta.append(m)
             muon_update(weights, grads, momenta, group["lr"], group["momentum"], group["nesterov"], group["weight_decay"],
                         group["steps"], group["coefficients"], group["eps"], group["scale"], precision=group["precision"])
         return loss

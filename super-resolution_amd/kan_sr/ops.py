@@ -195,7 +195,11 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}          # KSR_ACT_* 
 def _pixel_rows(t: torch.Tensor):
     """t [B, ..., C] -> (t or a dense copy, image stride, pixel stride, pixels): in place where the channels are contiguous
     and the middle dimensions are one run of pixels (dense tensors, channel slices, images of a larger buffer)."""
-    B, C, mid = t.shape[0], t.shape[-1], list(zip(t.shape[1:-1], t.stride()[1:-1]))
+    B, C, n = t.shape[0], t.shape[-1], t.numel()
+    if n and t.is_contiguous():
+        S = n // (B * C)
+        return t, S * C if B > 1 else 0, C if S > 1 else 0, S
+    mid = list(zip(t.shape[1:-1], t.stride()[1:-1]))
     S = 1
     for n, _ in mid:
         S *= n
