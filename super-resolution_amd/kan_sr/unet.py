@@ -711,6 +711,11 @@ class UNet(nn.Module):
         x = y_plane.contiguous()
         names, params = self._named_params()
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)):
+            if self.grad_sink is not None:
+                # The gradients go to the sink, past autograd: one leaf of this call's own keeps the tape alive.  The parameters
+                # themselves may belong to another graph that is still alive, whose stream autograd would then wait for: not
+                # possible while this backward is being recorded on a stream of its own.
+                params = [torch.empty(0, device=x.device, requires_grad=True)]
             return _UNetFn.apply(x, self, names, fuse_head, *params)
         with torch.no_grad():
             return self._run(x, self.training, None, fuse_head)
@@ -728,7 +733,7 @@ class _UNetFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, net, names, fuse_head, *params):
-        ctx.net, ctx.names, ctx.tape = net, names, {}
+        ctx.net, ctx.names, ctx.tape, ctx.leaves = net, names, {}, len(params)
         return net._run(x, net.training, ctx.tape, fuse_head)
 
     @staticmethod
@@ -739,6 +744,6 @@ class _UNetFn(torch.autograd.Function):
         gx = None
         if want_gx:         # [B,H,W,1] is [B,1,H,W]
             gx, ctx.net._input_grad = ctx.net._input_grad.view(-1, 1, *ctx.net._input_grad.shape[1:3]), None
-        if ctx.net.grad_sink is not None:
-            return (gx,) + (None,) * (3 + len(ctx.names))
+        if ctx.net.grad_sink is not None or ctx.leaves != len(ctx.names):
+            return (gx,) + (None,) * (3 + ctx.leaves)
         return (gx, None, None, None) + tuple(grads[n].contiguous() for n in ctx.names)

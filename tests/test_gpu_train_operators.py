@@ -210,6 +210,23 @@ def test_captured_muon_step_equals_launched_step(backbone):
     assert runs[0][0] == runs[1][0] and torch.equal(runs[0][1], runs[1][1]) and torch.equal(runs[0][2], runs[1][2])
 
 
+def test_recorded_while_an_eager_graph_of_the_parameters_lives():
+    from kan_sr.train import TrainStep
+    runs = []
+    for keep in (False, True):
+        torch.manual_seed(35)
+        m = _model().cuda()
+        gen = torch.Generator().manual_seed(9)
+        x0 = torch.rand(2, 3, 32, 32, generator=gen).cuda()
+        alive = m(x0) if keep else None
+        ts = TrainStep(m, lr=1e-3, optimizer="muon", capture=True)
+        for it in range(5):
+            ts.step(torch.rand(2, 3, 32, 32, generator=gen).cuda(), torch.rand(2, 3, 64, 64, generator=gen).cuda())
+        assert ts._graph is not None and (alive is None or alive.requires_grad)
+        runs.append((ts.flat_p.clone(), ts.exp_avg.clone()))
+    assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1])
+
+
 def test_changed_momentum_is_not_replayed_from_an_old_graph():
     from kan_sr.module import ConvSepKan
     from kan_sr.train import TrainStep
