@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
 }
 
 // One product of a step, C[i][j] = sum_k P[i][k] Q[j][k], and what follows it:
-//   A_OF_X      P = Q = X, tiles of the lower triangle:   R = A - diag A (both triangles), d = diag A
+//   A_OF_X      P = Q = X, tiles of the lower triangle:   R = A - diag A (exactly symmetric), d = diag A
 //   B_OF_A      P = Q = R, tiles of the lower triangle:   B - diag B, e = a + diag B
 //   X_NEXT      P = B, Q = X^T:                            X, X^T
 //   X_LAST      the same, result or weight update; TALL: P = X^T, Q = B, so that lanes run along U's rows either way
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
     constexpr int PBYTES = TM * BK * 2, QBYTES = TN * BK * 2, STAGE = NP * (PBYTES + QBYTES);
     constexpr int HALVES = NST * STAGE >= TM * (TN + 8) * 2 && NST * STAGE >= TN * (TM + 8) * 2 ? 1 : 2;      // the output tile reuses the stages
     static_assert(NST * STAGE >= TM / HALVES * (TN + 8) * 2 && NST * STAGE >= TN * (TM / HALVES + 8) * 2 && TM / HALVES >= WM, "output tile");
-    static_assert(TM == TN || KIND == X_NEXT || KIND == X_LAST, "a triangle of square tiles");
+    static_assert((TM == TN && !WIDE && HALVES == 1) || KIND == X_NEXT || KIND == X_LAST, "a triangle of square tiles that fit the stages");
     __shared__ __attribute__((aligned(16))) char lds[NST * STAGE];
     __shared__ int arrived;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / WC, wc = wave % WC;
@@ -918,7 +918,6 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                         v[z] *= S;
                     }
                 } else if constexpr (KIND == B_OF_A) {
-                    if (WIDE && row0 - ti * TM >= rows) continue;
                     const h4 rh = *reinterpret_cast<const h4*>(R + place(l.mp, c, row0));       // R is symmetric
                     h4 rl = {};
                     if constexpr (SPLIT) rl = *reinterpret_cast<const h4*>(R + pp + place(l.mp, c, row0));
@@ -1023,14 +1022,22 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
                 for (int w = threadIdx.x; w < HM * TN / 8; w += TH) {
                     const int r = (w >> 2) % height, c = (w >> 2) / height * 32 + (w & 3) * 8;        // along a block of 32 columns
                     const int i = tr ? c : r, j = tr ? r : c;        // row and column of the product's tile
-                    // what lies beyond an odd number of 128s is not stored; of a symmetric product, nothing above the diagonal's
-                    // blocks of TN, and the transposes of those below it
-                    bool ok = !WIDE || (half * HM + i < rows && j < cols);
+                    _Float16* to = o + place(of_rows, (tr ? j0 : i0) + r, (tr ? i0 : j0) + c);
                     if constexpr (SYM) {
-                        const int bi = (i0 + i) / TN;
-                        ok = ok && (tr ? bi > tj : bi >= tj);
-                    }
-                    if (ok) *reinterpret_cast<uint4*>(o + place(of_rows, (tr ? j0 : i0) + r, (tr ? i0 : j0) + c)) = *reinterpret_cast<const uint4*>(stage + r * pitch + c);
+                        // Above the diagonal stand the transposes of what is below it, in the diagonal's own tiles too: what these
+                        // computed there has hi lo and lo hi added in the other order, and where they end depends on the tile
+                        if (ti == tj) {
+                            if (tr ? c <= r : c > r) continue;
+                            if (SPLIT && !tr && c + 7 > r) {            // eight columns across the diagonal
+                                h8 v;
+#pragma unroll
+                                for (int z = 0; z < 8; ++z) v[z] = stage[(c + z > r ? c + z : r) * pitch + (c + z > r ? r : c + z)];
+                                *reinterpret_cast<h8*>(to) = v;
+                                continue;
+                            }
+                        }
+                    } else if (WIDE && !(half * HM + i < rows && j < cols)) continue;      // beyond an odd number of 128s
+                    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(stage + r * pitch + c);
                 }
                 ksr_lds_barrier();
             }
