@@ -793,7 +793,8 @@ int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t x_pixel_st
  * muon = 1 (fp32): g = grad_scale * src, momentum = momentum_factor * momentum + g, U = g + momentum_factor * momentum
  *   (nesterov) or momentum;  dst = (1 - lr weight_decay) dst - lr scale sqrt(max(rows, cols)) X.  momentum, dst dense.
  * split != 0: products of f16 pairs (22 bits), as close to 64 bits as fp32 arithmetic; 0: single f16 operands (diagonals and
- *   the linear term apart), about 1e-3 off, for bf16 results.
+ *   the linear term apart), 2e-4 to 9e-4 off, for bf16 results.  Either way a matrix's result does not depend on what else is
+ *   in the call.
  * mats: HOST array, read during the call.  src may have any non-negative element strides; src and dst may be the same memory.
  * Nothing that one matrix of a call writes (dst, momentum) may overlap what another reads or writes.  lr_dev: NULL, or a device float that replaces lr (recorded
  * graphs).  ws: ksr_muon_ws_bytes bytes of device memory, 16-byte aligned, free again when the call's kernels have run; calls

@@ -666,11 +666,14 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
 // Rows of a stage hold 16-byte chunks in an order that depends on the row (chunk c of row r at c ^ f(r)), so that the eight lanes
 // that read at once hit all banks.
 // Sums: along k in chunks of `chunk_of` columns; a chunk's sum is added to the tile's in the order of k.  Shorter chains of
-// roundings, and the result does not depend on who computes which chunk:
+// roundings, and the result does not depend on who computes which chunk.  X of single operands has one chain instead (the
+// 256 x 256 tile has no registers for a second sum) and is never cut, so that a tile of any size gives the same bits (bf16 against
+// chains and cuts that followed the tile: 2100 x 2100 602 us for 554, 2560 x 2560 723 for 864, 1536 x 1536 339 for 369).
 // Work split: of T tiles the first `whole` = 256 floor(T / 256) have a workgroup each; each chunk of the others has one of its
 // own (`cut`), so that a round that is not full still occupies the chip (528 tiles would otherwise take as long as 768).  Such a
 // workgroup leaves its fp32 sums in the workspace; the one that arrives last adds them in order and goes on with the tile.
 enum { A_OF_X, B_OF_A, X_NEXT, X_LAST };
+template <bool SPLIT, int KIND> constexpr bool folds() { return SPLIT || KIND == A_OF_X || KIND == B_OF_A; }
 
 // 512 columns, more where there would be over 64 chunks; of the unpadded length, so that the tile makes no difference
 __host__ __device__ inline int chunk_of(int k) {
@@ -698,7 +701,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
     __shared__ __attribute__((aligned(16))) char lds[NST * STAGE];
     __shared__ int arrived;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / WC, wc = wave % WC;
-    constexpr bool SYM = KIND == A_OF_X || KIND == B_OF_A;
+    constexpr bool SYM = KIND == A_OF_X || KIND == B_OF_A, FOLD = folds<SPLIT, KIND>();
     int t, slice = 0, slices = 1, slot = 0, q = 0;      // slot: of the tile's first partial sums
     if ((int)blockIdx.x < a.whole) {
         t = (int)ksr_xcd_contiguous(blockIdx.x, (unsigned)a.whole);
@@ -783,7 +786,7 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
         const int chunk = (2 * ks + (lane >> 5)) ^ f(row);
         return *reinterpret_cast<const h8*>(lds + st * STAGE + at_byte + row * (BK * 2) + 16 * chunk);
     };
-    f32x16 acc[MT][NT] = {}, sum[SPLIT ? MT : 1][SPLIT ? NT : 1] = {};
+    f32x16 acc[MT][NT] = {}, sum[FOLD ? MT : 1][FOLD ? NT : 1] = {};
     const int chunk = chunk_of(KIND == A_OF_X ? l.n : l.m) / BK, nk = K / BK;
     const int k0 = slices > 1 ? slice * chunk : 0, k1 = slices > 1 && k0 + chunk < nk ? k0 + chunk : nk;
     h8 ph[2][MT], qh[2][NT], pl[2][SPLIT ? MT : 1], ql[2][SPLIT ? NT : 1];
@@ -812,43 +815,46 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, TM / WM * (TN / WN) 
     for (int kt = k0; kt < k0 + NST - 1 && kt < k1; ++kt) fill(kt);
     stage_ready(k0);
     load(0, k0, 0);
-    for (int kt = k0; kt < k1; ++kt) {
+    for (int c0 = k0; c0 < k1; c0 += chunk) {           // k0 is the start of a chunk
+        const int c1 = FOLD && c0 + chunk < k1 ? c0 + chunk : k1;
+        for (int kt = c0; kt < c1; ++kt)
 #pragma unroll
-        for (int ks = 0; ks < BK / 16; ++ks) {
-            const int set = ks & 1;
-            if (ks + 1 < BK / 16) load(set ^ 1, kt, ks + 1);
-            else if (kt + 1 < k1) {
-                stage_ready(kt + 1);
-                load(set ^ 1, kt + 1, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int x = 0; x < MT; ++x)
-#pragma unroll
-                for (int y = 0; y < NT; ++y) {
-                    if constexpr (SPLIT) {
-                        acc[x][y] = mfma(ph[set][x], ql[set][y], acc[x][y]);
-                        acc[x][y] = mfma(pl[set][x], qh[set][y], acc[x][y]);
-                    }
-                    acc[x][y] = mfma(ph[set][x], qh[set][y], acc[x][y]);
+            for (int ks = 0; ks < BK / 16; ++ks) {
+                const int set = ks & 1;
+                if (ks + 1 < BK / 16) load(set ^ 1, kt, ks + 1);
+                else if (kt + 1 < k1) {
+                    stage_ready(kt + 1);
+                    load(set ^ 1, kt + 1, 0);
                 }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (SPLIT && (((kt + 1) & (chunk - 1)) == 0 || kt + 1 == k1))      // chunk is a power of two
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < MT; ++x)
+#pragma unroll
+                    for (int y = 0; y < NT; ++y) {
+                        if constexpr (SPLIT) {
+                            acc[x][y] = mfma(ph[set][x], ql[set][y], acc[x][y]);
+                            acc[x][y] = mfma(pl[set][x], qh[set][y], acc[x][y]);
+                        }
+                        acc[x][y] = mfma(ph[set][x], qh[set][y], acc[x][y]);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        if constexpr (!FOLD) break;
+        else
 #pragma unroll
             for (int x = 0; x < MT; ++x)
 #pragma unroll
                 for (int y = 0; y < NT; ++y) {
-                    sum[SPLIT ? x : 0][SPLIT ? y : 0] += acc[x][y];
+                    sum[x][y] += acc[x][y];
                     acc[x][y] = f32x16{};
                 }
     }
-    if constexpr (SPLIT)
+    if constexpr (FOLD)
 #pragma unroll
         for (int x = 0; x < MT; ++x)
 #pragma unroll
             for (int y = 0; y < NT; ++y) acc[x][y] = sum[x][y];
-    if (!WIDE && slices > 1) {
+    if (FOLD && slices > 1) {
         int* counter = reinterpret_cast<int*>(a.l.ws + a.l.o_part) + slot;
         float* part = reinterpret_cast<float*>(a.l.ws + a.l.o_part + 4l * COUNTERS) + (long)slot * TM * TN + threadIdx.x;
         float* own = part + (long)slice * TM * TN;
@@ -1150,8 +1156,8 @@ template <int TM, int TN, int WM, int WN, int BK, int NST, bool SPLIT, int KIND>
         if (n > 0) cut += (long)n * ((kp + ch - 1) / ch);
     }
     // Cut only what is worth its traffic: four chunks or more, or fewer tiles than CUs (429 tiles of 832 columns in two chunks: 20 us,
-    // uncut 14 us), and no tiles of 256 x 256
-    a.cut = TM * TN <= 128 * 128 && cut <= COUNTERS && cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile && (tiles < CUS || cut >= 4l * (tiles - a.whole));
+    // uncut 14 us), and no single chains (see above)
+    a.cut = folds<SPLIT, KIND>() && cut <= COUNTERS && cut * TM * TN <= (long)SLOTS * a.l.tile * a.l.tile && (tiles < CUS || cut >= 4l * (tiles - a.whole));
     hipLaunchKernelGGL((ns_gemm_kernel<TM, TN, WM, WN, BK, NST, SPLIT, KIND>), dim3((unsigned)(a.cut ? a.whole + cut : tiles)), dim3(TM / WM * (TN / WN) * 64), 0, st, a);
 }
 

@@ -20,3 +20,26 @@ def test_fp32_results_do_not_depend_on_the_rest_of_a_batch(shape, n):
     alone = newton_schulz(u)
     y = newton_schulz(u.expand(n, *shape))
     assert all(torch.equal(y[k], alone) for k in range(n))
+
+
+@pytest.mark.parametrize("shape,n", BATCHES)
+def test_bf16_results_do_not_depend_on_the_rest_of_a_batch(shape, n):
+    """Sums of single operands end in the same bits however the tiles are cut and whatever their size."""
+    from kan_sr.muon import newton_schulz
+    u = randn(*shape).bfloat16()
+    alone = newton_schulz(u)
+    y = newton_schulz(u.expand(n, *shape))
+    assert all(torch.equal(y[k], alone) for k in range(n))
+
+
+@pytest.mark.parametrize("precision", ["fp32", "bf16"])
+def test_lists_of_large_matrices_are_updated_like_their_entries(precision):
+    from kan_sr.muon import muon_update
+    shapes = [(777, 2051), (1536, 1536), (100, 600), (1500, 1400), (300, 3000), (1536, 1536), (900, 70), (2051, 777)]
+    w0, gs = [randn(*s, seed=k) for k, s in enumerate(shapes)], [1e-3 * randn(*s, seed=50 + k) for k, s in enumerate(shapes)]
+    W, M = [t.clone() for t in w0], [torch.zeros_like(t) for t in w0]
+    muon_update(W, gs, M, lr=0.02, precision=precision)
+    for w, g, a, b in zip(w0, gs, W, M):
+        m = torch.zeros_like(w)
+        muon_update([w], [g], [m], lr=0.02, precision=precision)
+        assert torch.equal(w, a) and torch.equal(m, b), tuple(w.shape)
