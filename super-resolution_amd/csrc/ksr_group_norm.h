@@ -13,6 +13,7 @@ struct GnArgs {
     long xs_b, xs_p, ds_b, ds_p;                       // image and pixel strides of x, dy in elements
     long B, S, chunk, nchunk;
     int C, G, Cg, CB, nblk, GB, CV, PL;                // channels per block, blocks, group slots per block, vectors, pixel lanes
+    int all;                                           // backward: these are all images of the call, not a range of them
     int past;                                          // write the result past the caches
     int join;                                          // the pass that uses the chunks' results joins them itself
     float eps;

@@ -616,6 +616,7 @@ template <class T, int VEC> int run_fwd(GnArgs& a, int act, hipStream_t st) {
 
 template <class T, int VEC, int ACT> int run_bwd_act(GnArgs& a, hipStream_t st) {
     split(a, VEC, in_flight<T, VEC>() / 2, true);
+    if (!a.all) a.join = 0;                             // the images' channel sums are needed beyond this launch
     const dim3 block(THREADS);
     const long work = a.B * a.nblk * a.nchunk;
     hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, VEC, ACT>), dim3((unsigned)work), block, 0, st, a);
@@ -626,7 +627,7 @@ template <class T, int VEC, int ACT> int run_bwd_act(GnArgs& a, hipStream_t st) 
         hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * a.G)), block, 0, st, a, tc);
         KSR_LAUNCH_CHECK("group_norm_bwd");
     }
-    const long wgs = (a.out ? work : 0) + (a.dw || a.db ? params_wgs(a.C) : 0);
+    const long wgs = (a.out ? work : 0) + (a.all && (a.dw || a.db) ? params_wgs(a.C) : 0);
     if (wgs) {
         if (a.past) hipLaunchKernelGGL((gn_bwd_dx_kernel<T, VEC, ACT, true>), dim3((unsigned)wgs), block, 0, st, a);
         else hipLaunchKernelGGL((gn_bwd_dx_kernel<T, VEC, ACT, false>), dim3((unsigned)wgs), block, 0, st, a);
@@ -643,11 +644,31 @@ template <class T, int VEC> int run_bwd(GnArgs& a, int act, hipStream_t st) {
     }
 }
 
+// A launch holds fewer than 2^32 threads.  No kernel has more workgroups per image than max(G, C / 256), beyond the few thousand of
+// small batches; they have 256 threads, 1024 only where a group of an image has more than 256 values.
+long images_at_once(int64_t S, int C, int G) {
+    const long threads = S > 256 || S * (C / G) > 256 ? 1024 : 256, per = G > (C + 255) / 256 ? G : (C + 255) / 256;
+    return ((1l << 32) / threads - 1 - 4096) / per;
+}
+
 int check_shape(const char* what, int64_t B, int64_t S, int C, int G) {
     KSR_CHECK_ARG(B >= 0 && S >= 0 && C > 0 && G > 0 && C % G == 0, "%s: [%lld, %lld, %d] in %d groups", what, (long long)B,
                   (long long)S, C, G);
     KSR_UNSUPPORTED(B > (1 << 24) || S > (1ll << 40) || B * (int64_t)G > (1ll << 30) || B * ((C + 255) / 256) > (1ll << 30),
                     "%s: [%lld, %lld, %d] is beyond the launch limits", what, (long long)B, (long long)S, C);
+    KSR_UNSUPPORTED(images_at_once(S, C, G) < 1, "%s: an image [%lld, %d] in %d groups is beyond the launch limits", what, (long long)S, C, G);
+    return KSR_OK;
+}
+
+// the images in as many equal ranges as images_at_once() asks for: images of a range, f(first image, images) for each
+long range_of(int64_t B, int64_t S, int C, int G) {
+    const long most = images_at_once(S, C, G), n = (B + most - 1) / most;
+    return (B + n - 1) / n;
+}
+template <class F> int for_ranges(int64_t B, int64_t S, int C, int G, F f) {
+    const long nb = range_of(B, S, C, G);
+    for (long b0 = 0; b0 < B; b0 += nb)
+        if (int rc = f(b0, nb < B - b0 ? nb : B - b0)) return rc;
     return KSR_OK;
 }
 
@@ -656,7 +677,13 @@ int check_shape(const char* what, int64_t B, int64_t S, int C, int G) {
 extern "C" int64_t ksr_group_norm_ws_floats(int64_t B, int64_t S, int C, int G, int backward) {
     if (check_shape("group_norm_ws_floats", B, S, C, G) != KSR_OK) return -1;
     if (B == 0 || S == 0) return 0;
-    return max_parts(B, S, C, G, backward != 0) + (backward ? 2 * B * G + 2 * B * C : 0);
+    int64_t most = 0;
+    for_ranges(B, S, C, G, [&](long, long n) {
+        const int64_t parts = max_parts(n, S, C, G, backward != 0);
+        if (parts > most) most = parts;
+        return KSR_OK;
+    });
+    return most + (backward ? 2 * B * G + 2 * B * C : 0);
 }
 
 extern "C" int ksr_group_norm_fwd(const void* x, int64_t x_image_stride, int64_t x_pixel_stride, const float* weight, const float* bias,
@@ -669,17 +696,21 @@ extern "C" int ksr_group_norm_fwd(const void* x, int64_t x_image_stride, int64_t
     KSR_CHECK_ARG(x && y && stats && ws, "group_norm_fwd: null pointer");
     KSR_CHECK_ARG(x_pixel_stride >= 0 && x_image_stride >= 0, "group_norm_fwd: negative stride");
     KSR_CHECK_ARG(aligned(x, bf16 ? 2 : 4) && aligned(y, bf16 ? 2 : 4), "group_norm_fwd: misaligned pointer");
-    GnArgs a{};
-    a.x = x; a.out = y; a.w = weight; a.b = bias; a.stats = stats; a.part = ws;
-    a.xs_b = x_image_stride; a.xs_p = x_pixel_stride;
-    a.B = B; a.S = S; a.C = C; a.G = G; a.Cg = C / G; a.eps = eps;
-    a.past = B * S * C * (bf16 ? 2 : 4) >= PAST_BYTES;
-    int vec, ne;
-    if (ksr_gn_one_fits(a, bf16 ? 2 : 4, false, vec, ne)) return ksr_gn_one_fwd(a, act, bf16 != 0, vec, ne, stream);
-    vec = vec_of(a, bf16 ? 2 : 4, false);
-    if (bf16)
-        return vec == 8 ? run_fwd<__bf16, 8>(a, act, stream) : vec == 4 ? run_fwd<__bf16, 4>(a, act, stream) : vec == 2 ? run_fwd<__bf16, 2>(a, act, stream) : run_fwd<__bf16, 1>(a, act, stream);
-    return vec == 4 ? run_fwd<float, 4>(a, act, stream) : vec == 2 ? run_fwd<float, 2>(a, act, stream) : run_fwd<float, 1>(a, act, stream);
+    const int es = bf16 ? 2 : 4;
+    return for_ranges(B, S, C, G, [&](long b0, long n) {
+        GnArgs a{};
+        a.x = reinterpret_cast<const char*>(x) + b0 * x_image_stride * es; a.out = reinterpret_cast<char*>(y) + b0 * S * C * es;
+        a.w = weight; a.b = bias; a.stats = stats + 2 * b0 * G; a.part = ws;
+        a.xs_b = x_image_stride; a.xs_p = x_pixel_stride;
+        a.B = n; a.S = S; a.C = C; a.G = G; a.Cg = C / G; a.eps = eps;
+        a.past = n * S * C * es >= PAST_BYTES;
+        int vec, ne;
+        if (ksr_gn_one_fits(a, es, false, vec, ne)) return ksr_gn_one_fwd(a, act, bf16 != 0, vec, ne, stream);
+        vec = vec_of(a, es, false);
+        if (bf16)
+            return vec == 8 ? run_fwd<__bf16, 8>(a, act, stream) : vec == 4 ? run_fwd<__bf16, 4>(a, act, stream) : vec == 2 ? run_fwd<__bf16, 2>(a, act, stream) : run_fwd<__bf16, 1>(a, act, stream);
+        return vec == 4 ? run_fwd<float, 4>(a, act, stream) : vec == 2 ? run_fwd<float, 2>(a, act, stream) : run_fwd<float, 1>(a, act, stream);
+    });
 }
 
 extern "C" int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t x_pixel_stride, const void* dy, int64_t dy_image_stride,
@@ -688,13 +719,9 @@ extern "C" int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t
                                   hipStream_t stream) {
     if (int rc = check_shape("group_norm_bwd", B, S, C, G)) return rc;
     KSR_CHECK_ARG(act >= KSR_ACT_NONE && act <= KSR_ACT_GELU, "group_norm_bwd: activation %d", act);
-    GnArgs a{};
-    a.x = x; a.dy = dy; a.out = dx; a.w = weight; a.b = bias; a.stats = const_cast<float*>(stats); a.dw = dweight; a.db = dbias;
-    a.xs_b = x_image_stride; a.xs_p = x_pixel_stride; a.ds_b = dy_image_stride; a.ds_p = dy_pixel_stride;
-    a.B = B; a.S = S; a.C = C; a.G = G; a.Cg = C / G;
-    a.past = B * S * C * (bf16 ? 2 : 4) >= PAST_BYTES;
     if (B == 0 || S == 0) {                               // empty sums
-        a.B = 0;
+        GnArgs a{};
+        a.C = C; a.dw = dweight; a.db = dbias;
         if (!dweight && !dbias) return KSR_OK;
         hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)params_wgs(C)), dim3(THREADS), 0, stream, a);
         KSR_LAUNCH_CHECK("group_norm_bwd");
@@ -703,21 +730,36 @@ extern "C" int ksr_group_norm_bwd(const void* x, int64_t x_image_stride, int64_t
     KSR_CHECK_ARG(x && dy && stats && ws, "group_norm_bwd: null pointer");
     KSR_CHECK_ARG(x_pixel_stride >= 0 && x_image_stride >= 0 && dy_pixel_stride >= 0 && dy_image_stride >= 0, "group_norm_bwd: negative stride");
     KSR_CHECK_ARG(aligned(x, bf16 ? 2 : 4) && aligned(dy, bf16 ? 2 : 4) && aligned(dx, bf16 ? 2 : 4), "group_norm_bwd: misaligned pointer");
-    a.coef = ws;
-    a.chsum = a.coef + 2 * B * G;
-    a.part = a.chsum + 2 * B * C;
-    int vec, ne;
-    if (ksr_gn_one_fits(a, bf16 ? 2 : 4, true, vec, ne)) {
-        if (!dweight && !dbias) a.chsum = nullptr;
-        if (int rc = ksr_gn_one_bwd(a, act, bf16 != 0, vec, ne, stream)) return rc;
-        if (B > 1 && a.chsum) {
-            hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)params_wgs(C)), dim3(THREADS), 0, stream, a);
-            KSR_LAUNCH_CHECK("group_norm_bwd");
+    const int es = bf16 ? 2 : 4;
+    float* const coef = ws;
+    float* const chsum = coef + 2 * B * G;
+    bool later = false;                                   // the parameters' gradients are left to be summed over the images
+    const int rc = for_ranges(B, S, C, G, [&](long b0, long n) {
+        GnArgs a{};
+        a.x = reinterpret_cast<const char*>(x) + b0 * x_image_stride * es; a.dy = reinterpret_cast<const char*>(dy) + b0 * dy_image_stride * es;
+        a.out = dx ? reinterpret_cast<char*>(dx) + b0 * S * C * es : nullptr;
+        a.w = weight; a.b = bias; a.stats = const_cast<float*>(stats) + 2 * b0 * G; a.dw = dweight; a.db = dbias;
+        a.xs_b = x_image_stride; a.xs_p = x_pixel_stride; a.ds_b = dy_image_stride; a.ds_p = dy_pixel_stride;
+        a.B = n; a.S = S; a.C = C; a.G = G; a.Cg = C / G;
+        a.past = n * S * C * es >= PAST_BYTES;
+        a.all = n == B;
+        a.coef = coef + 2 * b0 * G; a.chsum = chsum + 2 * b0 * C; a.part = chsum + 2 * B * C;
+        int vec, ne;
+        if (ksr_gn_one_fits(a, es, true, vec, ne)) {
+            if (!dweight && !dbias) a.chsum = nullptr;
+            later = B > 1 && a.chsum;
+            return ksr_gn_one_bwd(a, act, bf16 != 0, vec, ne, stream);
         }
-        return KSR_OK;
-    }
-    vec = vec_of(a, bf16 ? 2 : 4, true);
-    if (bf16)
-        return vec == 8 ? run_bwd<__bf16, 8>(a, act, stream) : vec == 4 ? run_bwd<__bf16, 4>(a, act, stream) : vec == 2 ? run_bwd<__bf16, 2>(a, act, stream) : run_bwd<__bf16, 1>(a, act, stream);
-    return vec == 4 ? run_bwd<float, 4>(a, act, stream) : vec == 2 ? run_bwd<float, 2>(a, act, stream) : run_bwd<float, 1>(a, act, stream);
+        later = !a.all && (dweight || dbias);
+        vec = vec_of(a, es, true);
+        if (bf16)
+            return vec == 8 ? run_bwd<__bf16, 8>(a, act, stream) : vec == 4 ? run_bwd<__bf16, 4>(a, act, stream) : vec == 2 ? run_bwd<__bf16, 2>(a, act, stream) : run_bwd<__bf16, 1>(a, act, stream);
+        return vec == 4 ? run_bwd<float, 4>(a, act, stream) : vec == 2 ? run_bwd<float, 2>(a, act, stream) : run_bwd<float, 1>(a, act, stream);
+    });
+    if (rc || !later) return rc;
+    GnArgs a{};
+    a.B = B; a.C = C; a.chsum = chsum; a.dw = dweight; a.db = dbias;
+    hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((unsigned)params_wgs(C)), dim3(THREADS), 0, stream, a);
+    KSR_LAUNCH_CHECK("group_norm_bwd");
+    return KSR_OK;
 }

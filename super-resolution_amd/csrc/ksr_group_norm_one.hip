@@ -218,8 +218,9 @@ __global__ void __launch_bounds__(TH) gn_one_bwd_kernel(GnArgs a) {
     }
     if (w.active && w.pl == 0) {
         // one image: these are the parameters' gradients
-        float* o1 = a.B == 1 ? a.db : a.chsum + 2 * w.b * a.C;
-        float* o2 = a.B == 1 ? a.dw : a.chsum + (2 * w.b + 1) * a.C;
+        const bool only = a.all && a.B == 1;
+        float* o1 = only ? a.db : a.chsum + 2 * w.b * a.C;
+        float* o2 = only ? a.dw : a.chsum + (2 * w.b + 1) * a.C;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             if (o1) o1[c + i] = d1[i];

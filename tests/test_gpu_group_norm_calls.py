@@ -1,0 +1,44 @@
+"""Group norm + activation (kan_sr.ops.group_norm_act) in calls of the largest numbers of groups."""
+import pytest
+import torch
+
+from test_gpu_group_norm import U32, formula, z_error
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("B,S,C,G", [((1 << 21) + 3, 2, 32, 8),            # 2^24 + 24 workgroups of 256 threads in one pass
+                                     ((1 << 20) + 1, 1, 64, 32)])          # a pixel per image: group norm per token, 2^25 groups
+def test_more_groups_than_one_launch_holds(B, S, C, G):
+    """2^32 threads are more than a launch takes: the images go in ranges."""
+    from kan_sr.ops import group_norm_act
+    g = torch.Generator("cuda").manual_seed(B)
+    x = torch.randn(B, S, C, device="cuda", generator=g)
+    w, b = 1 + 0.3 * torch.randn(C, device="cuda", generator=g), 0.3 * torch.randn(C, device="cuda", generator=g)
+    dy = torch.randn(B, S, C, device="cuda", generator=g)
+    args = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = group_norm_act(args[0], G, args[1], args[2], activation="silu")
+    dx, dw, db = torch.autograd.grad(y, args, dy)
+    # the first, the last and the images around the borders of ranges
+    some = torch.cat([torch.arange(k, k + 40) for k in (0, B // 4 - 20, B // 3 - 20, B // 2 - 20, 2 * B // 3 - 20, 3 * B // 4 - 20, B - 40)]).cuda()
+    x64, w64, b64 = x[some].double().requires_grad_(), w.double().requires_grad_(), b.double().requires_grad_()
+    y64, xhat, z, mean, rstd = formula(x64, w64, b64, G, 1e-5, "silu")
+    y64.backward(dy[some].double())
+    with torch.no_grad():
+        ez = z_error(x64, w64, b64, xhat, z, mean, rstd)
+        assert bool(((y[some].double() - y64).abs() <= 1.2 * ez + 16 * U32 * (z.abs() + 1)).all())
+        # dx: three terms of dz and xhat, each with ez and a few dozen roundings of values of at most |w dz| (1 + |xhat|) rstd
+        size = rstd * (1 + xhat.abs()) ** 2 * (w64.abs().max() + 1) * dy[some].double().abs().amax(dim=(1, 2), keepdim=True)
+        assert bool(((dx[some].double() - x64.grad).abs() <= size * (4 * ez.amax(dim=(1, 2), keepdim=True) + 256 * U32)).all())
+        # dw, db: of all images, in 64 bits part by part; at most B S / 4 + 64 roundings of the sums of absolute values
+        ref, total = torch.zeros(2, C, dtype=torch.float64, device="cuda"), torch.zeros(2, C, dtype=torch.float64, device="cuda")
+        for lo in range(0, B, 1 << 18):
+            p, d = x[lo:lo + (1 << 18)].double(), dy[lo:lo + (1 << 18)].double()
+            _, xh, zz, _, _ = formula(p, w.double(), b.double(), G, 1e-5, "silu")
+            s = torch.sigmoid(zz)
+            dz = d * s * (1 + zz * (1 - s))
+            for k, t in enumerate((dz, dz * xh)):
+                ref[k] += t.sum(dim=(0, 1))
+                total[k] += t.abs().sum(dim=(0, 1))
+        tol = (B * S / 4 + 64) * U32 * total + 64 * U32 * total
+        assert bool(((torch.stack([db, dw]).double() - ref).abs() <= tol).all())

@@ -128,3 +128,16 @@ def test_group_norm_unet_has_the_batch_norm_keys_without_running_statistics():
     batch, group = UNet(1, 40).state_dict(), UNet(1, 40, norm="group").state_dict()
     assert set(group) == {k for k in batch if "running" not in k and "num_batches" not in k}
     assert all(group[k].shape == batch[k].shape for k in group)
+
+
+def test_group_norm_limits_of_an_image():
+    from kan_sr import _lib
+    L = _lib.lib()
+
+    def ws(B, S, C, G):
+        return L.ksr_group_norm_ws_floats(c_int64(B), c_int64(S), c_int(C), c_int(G), c_int(0))
+
+    # 2^32 threads and more in a launch: images in ranges, one image's groups have to fit
+    assert ws(1 << 20, 1, 512, 32) > 0 and ws(1 << 23, 2, 8, 8) > 0
+    assert ws(1, 2, 1 << 23, 1 << 23) > 0 and ws(1, 300, 1 << 23, 1 << 23) == -1 and b"launch limits" in L.ksr_last_error()
+    assert ws(1, 2, 1 << 25, 1 << 25) == -1
