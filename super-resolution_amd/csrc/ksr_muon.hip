@@ -25,6 +25,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float S = 1024.f, INV_S = 1.f / 1024.f;     // values up to 30 (checked on the host) fit f16
 constexpr int MAX_STEPS = 32, MAX_MATS = 40;
+constexpr int SMALL_WGS = 1 << 22;                    // workgroups (of 512 threads) of a launch: it holds fewer than 2^32 threads
 
 struct Mat {
     const void* src;          // U, or the gradient
@@ -32,6 +33,7 @@ struct Mat {
     float* mom;               // Muon: momentum (fp32, dense)
     long rs, cs, bs;          // strides of src in elements: row, column, matrix
     int rows, cols, batch, first;
+    int sub0;                 // small matrices: index in the batch of the launch's first one
 };
 
 struct Step {
@@ -46,7 +48,7 @@ struct Mats { Mat m[MAX_MATS]; int count; Step s; };
 __device__ __forceinline__ const Mat& find(const Mats& p, int i, int& sub) {
     int k = 0;
     while (k + 1 < p.count && i >= p.m[k + 1].first) ++k;
-    sub = i - p.m[k].first;
+    sub = p.m[k].sub0 + i - p.m[k].first;
     return p.m[k];
 }
 
@@ -1096,7 +1098,7 @@ long next_group(const KsrMatrix* mats, int count, bool split, int& entry, int& s
             e.parts = elements / 4096 < 1 ? 1 : elements / 4096 < NORM_PARTS ? (int)(elements / 4096) : NORM_PARTS;
             e.off = off;
             e.first = matrices;
-            m[l.count++] = Mat{k.src, k.dst, k.momentum, (long)k.row_stride, (long)k.col_stride, (long)k.batch_stride, k.rows, k.cols, k.batch, 0};
+            m[l.count++] = Mat{k.src, k.dst, k.momentum, (long)k.row_stride, (long)k.col_stride, (long)k.batch_stride, k.rows, k.cols, k.batch, 0, 0};
             off += e.nsub * per;
             matrices += e.nsub;
             full += e.nsub * mt * nt;
@@ -1261,19 +1263,17 @@ extern "C" int ksr_muon_batch(const KsrMatrix* mats, int count, int bf16, int sp
     KSR_CHECK_ARG(ws_bytes >= ksr_muon_ws_bytes(mats, count, split), "muon_batch: the workspace has %lld bytes, %lld are needed",
                   (long long)ws_bytes, (long long)ksr_muon_ws_bytes(mats, count, split));
     KSR_CHECK_ARG((ws || ws_bytes == 0) && reinterpret_cast<uintptr_t>(ws) % 16 == 0, "muon_batch: null or misaligned workspace");
-    auto add = [&](const KsrMatrix& q, int first) {
-        Mat& m = p.m[p.count++];
-        m = Mat{q.src, q.dst, q.momentum, (long)q.row_stride, (long)q.col_stride, (long)q.batch_stride, q.rows, q.cols, q.batch, first};
-    };
-    auto small = [&](const KsrMatrix& q) { return is_small(q.rows, q.cols); };
-    // every small matrix of the list in one launch (of up to MAX_MATS entries)
-    for (int i = 0; i < count;) {
+    // every small matrix of the list in one launch, of up to MAX_MATS entries and SMALL_WGS matrices; `sub`: what of entry i is done
+    for (int i = 0, sub = 0; i < count;) {
         p.count = 0;
-        int64_t total = 0;
-        for (; i < count && p.count < MAX_MATS; ++i) {
-            if (empty(mats[i]) || !small(mats[i])) continue;
-            add(mats[i], (int)total);
-            total += mats[i].batch;
+        int total = 0;
+        for (; i < count && p.count < MAX_MATS && total < SMALL_WGS; ++i, sub = 0) {
+            const KsrMatrix& q = mats[i];
+            if (empty(q) || !is_small(q.rows, q.cols)) continue;
+            const int left = q.batch - sub, n = left < SMALL_WGS - total ? left : SMALL_WGS - total;
+            p.m[p.count++] = Mat{q.src, q.dst, q.momentum, (long)q.row_stride, (long)q.col_stride, (long)q.batch_stride, q.rows, q.cols, q.batch, total, sub};
+            total += n;
+            if (n < left) { sub += n; break; }
         }
         if (!p.count) continue;
         const int mode = mode_of(p.s);

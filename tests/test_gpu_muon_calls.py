@@ -43,3 +43,19 @@ def test_lists_of_large_matrices_are_updated_like_their_entries(precision):
         m = torch.zeros_like(w)
         muon_update([w], [g], [m], lr=0.02, precision=precision)
         assert torch.equal(w, a) and torch.equal(m, b), tuple(w.shape)
+
+
+def test_more_small_matrices_than_one_launch_holds():
+    """2^22 workgroups of 512 threads run together, the rest of the batch in the next launches."""
+    from kan_sr.muon import newton_schulz
+    n = (1 << 23) + 3                                  # of 2^32 threads and more a launch is invalid
+    u = randn(n, 1, 2)
+    y = newton_schulz(u, steps=1)
+    x = u.double() / (u.double().norm(dim=(1, 2), keepdim=True) + 1e-7)
+    a, b, c = 3.4445, -4.7750, 2.0315
+    A = x.square().sum(dim=2, keepdim=True)
+    ref = (a + b * A + c * A * A) * x
+    # operands of 22 bits: three products of a few units of 2^-22 each, of values of at most 3.4445 + 4.775 + 2.0315
+    assert float((y.double() - ref).abs().max()) <= 4 * (a - b + c) * 2.0 ** -22
+    for k in (0, (1 << 22) - 1, 1 << 22, n - 1):
+        assert torch.equal(newton_schulz(u[k], steps=1), y[k])
