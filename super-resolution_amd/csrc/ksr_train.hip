@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(256) adam_runs_kernel(AdamRuns r, float* __res
         lr = *lr_dev;
     }
     const long first = r.first[blockIdx.y];
-    for (int k = (int)(blockIdx.x * blockDim.x + threadIdx.x); k < r.len[blockIdx.y]; k += (int)(gridDim.x * blockDim.x)) {
+    // 64 bits: a step may pass the end of a run of almost 2^31 elements
+    for (long k = (long)blockIdx.x * blockDim.x + threadIdx.x; k < r.len[blockIdx.y]; k += (long)gridDim.x * blockDim.x) {
         const long i = first + k;
         float gi = g[i] * gscale;
         const float pi = p[i];
