@@ -12,6 +12,7 @@ from contextlib import nullcontext
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p, POINTER
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libksr.so")
@@ -158,6 +159,13 @@ def on_device_of(t: torch.Tensor):
     if _RAW_DEVICE is not None and _RAW_DEVICE() == t.device.index:
         return nullcontext()
     return torch.cuda.device(t.device)
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether a tensor carries a forward-mode tangent (of which `requires_grad` says nothing)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:          # no dual level is open: nothing to look at
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def host_floats(values) -> ctypes.Array:

@@ -11,7 +11,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import KsrError, check, host_floats, lib, on_device_of, ptr, stream
+from ._lib import KsrError, check, has_tangent, host_floats, lib, on_device_of, ptr, stream
 
 
 def make_knots(grid_size: int, spline_order: int, grid_range: Sequence[float]) -> list:
@@ -277,7 +277,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     and channels of a group of one image.  activation: "none", "relu", "silu" or "gelu" (the exact one).  x float32 or
     bfloat16, weight and bias [C] float32 or None; statistics and sums are fp32, the result has x's type and is dense.
     A channel slice of a wider tensor is read in place; of an NCHW tensor in torch.channels_last layout pass
-    x.permute(0, 2, 3, 1)."""
+    x.permute(0, 2, 3, 1).  Reverse mode only, once: forward-mode tangents raise."""
     if activation not in ACTIVATIONS:
         raise KsrError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
     if x.dim() < 2:
@@ -296,6 +296,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
             raise KsrError(f"group_norm_act: {name} must be float32 [{C}] on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    # past the autograd function only what nobody follows: it is what a trace records, and it raises for forward-mode tangents
+    if (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))
+            or torch.jit.is_tracing() or has_tangent(x, weight, bias)):
         return _GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation])
     return _group_norm_fwd(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation])[0]

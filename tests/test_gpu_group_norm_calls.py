@@ -1,4 +1,4 @@
-"""Group norm + activation (kan_sr.ops.group_norm_act) in calls of the largest numbers of groups."""
+"""Group norm + activation (kan_sr.ops.group_norm_act) in calls of the largest numbers of groups, traces and forward mode."""
 import pytest
 import torch
 
@@ -42,3 +42,31 @@ def test_more_groups_than_one_launch_holds(B, S, C, G):
                 total[k] += t.abs().sum(dim=(0, 1))
         tol = (B * S / 4 + 64) * U32 * total + 64 * U32 * total
         assert bool(((torch.stack([db, dw]).double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traced_calls_run_the_kernels():
+    from kan_sr.ops import group_norm_act
+    x = torch.randn(2, 30, 16, device="cuda")
+    w, b = torch.randn(16, device="cuda"), torch.randn(16, device="cuda")
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            traced = torch.jit.trace(lambda t: group_norm_act(t, 4, w, b, activation="silu"), (x,))
+            for k in range(2):
+                u = torch.randn(2, 30, 16, device="cuda")
+                assert torch.equal(traced(u), group_norm_act(u, 4, w, b, activation="silu"))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_is_refused_not_dropped(which):
+    from torch.autograd import forward_ad
+    from kan_sr.ops import group_norm_act
+    args = [torch.randn(2, 30, 16, device="cuda"), torch.randn(16, device="cuda"), torch.randn(16, device="cuda")]
+    plain = group_norm_act(args[0], 4, *args[1:])
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            assert torch.equal(group_norm_act(args[0], 4, *args[1:]), plain)          # nothing dual: an ordinary call
+            dual = list(args)
+            dual[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                group_norm_act(dual[0], 4, *dual[1:])
