@@ -12,7 +12,7 @@ from typing import Iterable, Optional, Sequence
 
 import torch
 
-from ._lib import KsrError, check, lib, on_device_of, stream
+from ._lib import KsrError, check, has_tangent, lib, on_device_of, stream
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MATRIX_WORDS = 8                                  # KsrMatrix of include/ksr.h as 64-bit words
@@ -68,9 +68,15 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
         raise KsrError("libksr ops need GPU tensors (the HIP path is the only path)")
     if g.dtype not in (torch.float32, torch.bfloat16):
         raise KsrError(f"newton_schulz: g must be float32 or bfloat16, got {g.dtype}")
-    if g.requires_grad and torch.is_grad_enabled():
+    if g.requires_grad and torch.is_grad_enabled() or has_tangent(g):
         raise KsrError("newton_schulz is not differentiable: detach g")
     split = _split(precision, g.dtype)
+    if torch.jit.is_tracing():                       # a trace records the call, not the allocation of its result alone
+        return _NewtonSchulz.apply(g, split, steps, coefficients, eps)
+    return _newton_schulz(g, split, steps, coefficients, eps)
+
+
+def _newton_schulz(g: torch.Tensor, split: bool, steps: int, coefficients, eps: float) -> torch.Tensor:
     out = torch.empty(g.shape, device=g.device, dtype=g.dtype)
     if g.numel() == 0:
         return out
@@ -82,6 +88,16 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
     bs, rs, cs = u.stride()
     _run(_matrix(u.data_ptr(), out.data_ptr(), 0, rs, cs, bs, rows, cols, batch), g, g.dtype is torch.bfloat16, split, steps, coefficients, eps)
     return out
+
+
+class _NewtonSchulz(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, split, steps, coefficients, eps):
+        return _newton_schulz(g, split, steps, coefficients, eps)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise KsrError("newton_schulz is not differentiable: detach g")
 
 
 def as_matrix(shape: Sequence[int]):
@@ -114,6 +130,8 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
     device = weights[0].device
     if device.type != "cuda":
         raise KsrError("libksr ops need GPU tensors (the HIP path is the only path)")
+    if torch.jit.is_tracing() or has_tangent(*weights, *grads, *momenta):
+        raise KsrError("muon_update works in place on plain tensors: it can be neither traced nor differentiated")
     f32 = torch.float32
     if lr_dev is not None and (lr_dev.dtype is not f32 or lr_dev.numel() != 1 or lr_dev.device != device):
         raise KsrError("muon_update: lr_dev must be one float32 on the weights' device")

@@ -1,4 +1,4 @@
-"""What else a call holds makes no difference to a matrix, and calls of the largest sizes (kan_sr.muon)."""
+"""What else a call holds makes no difference to a matrix; calls of the largest sizes, traces and forward mode (kan_sr.muon)."""
 import pytest
 import torch
 
@@ -59,3 +59,40 @@ def test_more_small_matrices_than_one_launch_holds():
     assert float((y.double() - ref).abs().max()) <= 4 * (a - b + c) * 2.0 ** -22
     for k in (0, (1 << 22) - 1, 1 << 22, n - 1):
         assert torch.equal(newton_schulz(u[k], steps=1), y[k])
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("shape", [(24, 40), (3, 100, 140)])
+def test_traced_calls_run_the_kernels(shape):
+    from kan_sr.muon import newton_schulz
+    traced = torch.jit.trace(lambda t: newton_schulz(t), (randn(*shape),))
+    for k in range(2):
+        u = randn(*shape, seed=10 + k)
+        assert torch.equal(traced(u), newton_schulz(u))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_forward_mode_and_traced_updates_are_refused_not_dropped():
+    from torch.autograd import forward_ad
+    from kan_sr._lib import KsrError
+    from kan_sr.muon import muon_update, newton_schulz
+    a, b, c = (randn(24, 40, seed=k) for k in range(3))
+    before = [t.clone() for t in (a, b, c)]
+    with forward_ad.dual_level():
+        assert torch.equal(newton_schulz(a), newton_schulz(a.clone()))              # nothing dual: an ordinary call
+        dual = forward_ad.make_dual(a, torch.ones_like(a))
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad):
+                with pytest.raises(KsrError, match="differentiable"):
+                    newton_schulz(dual)
+        for args in ((dual, b, c), (b, dual, c), (b, c, dual)):
+            with pytest.raises(KsrError, match="differentiated"):
+                muon_update(*([t] for t in args), lr=0.1)
+
+    def update(t):
+        muon_update([a], [t], [c], lr=0.1)
+        return a + t
+
+    with pytest.raises(KsrError, match="traced"):
+        torch.jit.trace(update, (b,))
+    assert all(torch.equal(t, u) for t, u in zip((a, b, c), before))
