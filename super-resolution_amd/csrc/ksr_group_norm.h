@@ -46,6 +46,10 @@ template <class T, int VEC> struct Vec {
     }
 };
 
+// What the activation is taken of, from xhat = (x - mean) * rstd: one expression for forward and backward, so that ReLU's mask is
+// that of the result (as fmaf(x - mean, w * rstd, b) a value next to 0 may have the other sign)
+__device__ __forceinline__ float gn_z(float xhat, float w, float b) { return fmaf(xhat, w, b); }
+
 template <int ACT> __device__ __forceinline__ float act_of(float z) {
     if constexpr (ACT == KSR_ACT_RELU) return z < 0.f ? 0.f : z;                // NaN stays NaN
     else if constexpr (ACT == KSR_ACT_SILU) return z * ksr_sigmoid(z);

@@ -253,9 +253,7 @@ __global__ void __launch_bounds__(THREADS) gn_apply_kernel(GnArgs a) {
     }
     if (!w.active) return;
     const int c = w.c0 + w.tv * VEC;
-    Affine<VEC> k(a, stats, c);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) k.w[i] *= k.rstd[i];
+    const Affine<VEC> k(a, stats, c);
     const T* src = reinterpret_cast<const T*>(a.x) + w.b * a.xs_b + c;
     T* dst = reinterpret_cast<T*>(a.out) + w.b * a.S * a.C + c;
     typename V::Raw next[R];
@@ -274,7 +272,7 @@ __global__ void __launch_bounds__(THREADS) gn_apply_kernel(GnArgs a) {
                 float v[VEC];
                 V::unpack(raw[r], v);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[i] = act_of<ACT>(fmaf(v[i] - k.mean[i], k.w[i], k.b[i]));
+                for (int i = 0; i < VEC; ++i) v[i] = act_of<ACT>(gn_z((v[i] - k.mean[i]) * k.rstd[i], k.w[i], k.b[i]));
                 put<V, PAST>(dst + (base + (long)r * a.PL) * a.C, V::pack(v));
             }
     }
@@ -312,7 +310,7 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_reduce_kernel(GnArgs a) {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
                         const float xh = (v[i] - k.mean[i]) * k.rstd[i];
-                        const float dz = g[i] * act_slope<ACT>(fmaf(xh, k.w[i], k.b[i]));
+                        const float dz = g[i] * act_slope<ACT>(gn_z(xh, k.w[i], k.b[i]));
                         d1[i] += dz;
                         d2[i] = fmaf(dz, xh, d2[i]);
                     }
@@ -508,7 +506,7 @@ __global__ void __launch_bounds__(THREADS) gn_bwd_dx_kernel(GnArgs a) {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     const float xh = (v[i] - k.mean[i]) * k.rstd[i];
-                    const float dz = g[i] * act_slope<ACT>(fmaf(xh, k.w[i], k.b[i]));
+                    const float dz = g[i] * act_slope<ACT>(gn_z(xh, k.w[i], k.b[i]));
                     v[i] = k.rstd[i] * (fmaf(dz, k.w[i], -q1[i]) - xh * q2[i]);
                 }
                 put<V, PAST>(dst + (base + (long)r * a.PL) * a.C, V::pack(v));

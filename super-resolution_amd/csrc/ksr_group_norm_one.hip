@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(TH) gn_one_fwd_kernel(GnArgs a) {
     float k[VEC], b[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-        k[i] = (a.w ? a.w[c + i] : 1.f) * rstd[i / PE];
+        k[i] = a.w ? a.w[c + i] : 1.f;
         b[i] = a.b ? a.b[c + i] : 0.f;
     }
     T* dst = reinterpret_cast<T*>(a.out) + w.b * a.S * a.C + c;
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(TH) gn_one_fwd_kernel(GnArgs a) {
             float v[VEC];
             V::unpack(raw[r], v);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = act_of<ACT>(fmaf(v[i] - mean[i / PE], k[i], b[i]));
+            for (int i = 0; i < VEC; ++i) v[i] = act_of<ACT>(gn_z((v[i] - mean[i / PE]) * rstd[i / PE], k[i], b[i]));
             *reinterpret_cast<typename V::Raw*>(dst + (long)(w.pl + r * w.PL) * a.C) = V::pack(v);
         }
 }
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(TH) gn_one_bwd_kernel(GnArgs a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             xh[i] = (xh[i] - mean[i / PE]) * rstd[i / PE];
-            dz[i] *= act_slope<ACT>(fmaf(xh[i], wt[i], bs[i]));
+            dz[i] *= act_slope<ACT>(gn_z(xh[i], wt[i], bs[i]));
         }
     };
 #pragma unroll

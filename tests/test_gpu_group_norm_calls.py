@@ -70,3 +70,25 @@ def test_forward_mode_is_refused_not_dropped(which):
             dual[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
             with pytest.raises((RuntimeError, NotImplementedError)):
                 group_norm_act(dual[0], 4, *dual[1:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,G", [((3, 200, 16), 4), ((2, 300, 24), 6), ((2, 60, 60, 90), 9), ((1, 130, 127, 320), 32), ((2, 400, 8), 4)])
+def test_relu_has_one_mask(shape, G, dtype):
+    """Values at the edge: every channel's bias is -w xhat of the values that half of its elements have, so that z is what rounding
+    leaves.  The gradient of the bias counts the positive results, exactly (dy = 1, fewer than 2^24 of them)."""
+    from kan_sr.ops import group_norm_act
+    g = torch.Generator().manual_seed(7)
+    C = shape[-1]
+    x = torch.randn(shape, generator=g)
+    level = torch.randn(C, generator=g)
+    x = torch.where(torch.rand(shape, generator=g) < 0.5, level.expand(shape), x).to(dtype)
+    w = 1 + 0.3 * torch.randn(C, generator=g)
+    _, xhat, _, _, _ = formula(x.double(), torch.ones(C, dtype=torch.float64), torch.zeros(C, dtype=torch.float64), G, 1e-5, "none")
+    edge = xhat[0].reshape(-1, C)[(x[0] == level.to(dtype)).reshape(-1, C).int().argmax(dim=0), torch.arange(C)]
+    b = (-(w.double() * edge)).float()
+    x, w, b = x.cuda().requires_grad_(), w.cuda().requires_grad_(), b.cuda().requires_grad_()
+    y = group_norm_act(x, G, w, b, activation="relu")
+    assert float((y.detach().float().reshape(-1, C)[(x.detach() == level.to(dtype).cuda()).reshape(-1, C).any(dim=1)]).min()) == 0.0
+    db, = torch.autograd.grad(y, (b,), torch.ones_like(y))
+    assert torch.equal(db, (y > 0).reshape(-1, C).sum(dim=0).float())
