@@ -7,7 +7,7 @@ is all this package's hyper-encoders have, run in one launch for the whole list.
 """
 from __future__ import annotations
 
-from ctypes import c_int64
+from array import array
 from typing import Iterable, Optional, Sequence
 
 import torch
@@ -24,11 +24,12 @@ def _matrix(src: int, dst: int, momentum: int, row_stride: int, col_stride: int,
     return src, dst, momentum, row_stride, col_stride, batch_stride, rows | cols << 32, batch
 
 
-def _run(words: list, device_of: torch.Tensor, bf16: bool, split: bool, steps: int, coefficients, eps: float, muon: bool = False,
+def _run(words: Sequence[int], device_of: torch.Tensor, bf16: bool, split: bool, steps: int, coefficients, eps: float, muon: bool = False,
          momentum: float = 0.0, nesterov: bool = False, grad_scale: float = 1.0, lr: float = 0.0,
          lr_dev: Optional[torch.Tensor] = None, weight_decay: float = 0.0, scale: float = 0.0) -> None:
     L = lib()
-    mats, n = (c_int64 * len(words))(*words), len(words) // MATRIX_WORDS
+    held, n = array("q", words), len(words) // MATRIX_WORDS
+    mats = held.buffer_info()[0]
     with on_device_of(device_of):
         nbytes = L.ksr_muon_ws_bytes(mats, n, split)
         if nbytes < 0:
@@ -119,7 +120,8 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
         m <- momentum m + grad_scale g;   U = grad_scale g + momentum m (nesterov) or m;   O = newton_schulz(U)
         w <- (1 - lr weight_decay) w - lr scale sqrt(max(rows, cols)) O
 
-    scale = 0.2 gives an update the root mean square of a typical Adam step, so that one learning rate serves both.  lr_dev: a
+    Nothing that is written (weights, momenta) may lie between the first and the last element of anything else in the call;
+    gradients may be views of each other.  scale = 0.2 gives an update the root mean square of a typical Adam step, so that one learning rate serves both.  lr_dev: a
     one-element float32 GPU tensor that replaces lr (recorded graphs)."""
     steps, coefficients = _steps_and_coefficients(steps, coefficients)
     weights, grads, momenta = list(weights), list(grads), list(momenta)
@@ -136,39 +138,43 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
     if lr_dev is not None and (lr_dev.dtype is not f32 or lr_dev.numel() != 1 or lr_dev.device != device):
         raise KsrError("muon_update: lr_dev must be one float32 on the weights' device")
     every = weights + grads + momenta
-    if {t.dtype for t in every} != {f32} or {t.get_device() for t in every} != {device.index}:
+    if {t.dtype for t in every} != {f32} or set(map(torch.Tensor.get_device, every)) != {device.index}:
         raise KsrError(f"muon_update: every weight, gradient and momentum must be float32 on {device}")
+    # methods mapped over lists: a call's time is the host's (every tensor's attributes in turn: 5 us more for 16 matrices)
+    T = torch.Tensor
+    shapes = list(map(T.size, weights))
+    if not (shapes == list(map(T.size, grads)) == list(map(T.size, momenta)) and all(map(T.is_contiguous, weights + momenta))):
+        i = next(i for i, (w, g, m) in enumerate(zip(weights, grads, momenta))
+                 if not w.shape == g.shape == m.shape or not w.is_contiguous() or not m.is_contiguous())
+        raise KsrError(f"muon_update: tensor {i}: gradient and momentum must have the weight's shape {tuple(shapes[i])}, weight "
+                       "and momentum be contiguous")
     words, held, spans = [], [], []
-    for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
-        shape = w.shape
-        if len(shape) < 2:
-            raise KsrError(f"muon_update: tensor {i} is {tuple(shape)}: matrices only (vectors belong to Adam)")
-        if g.shape != shape or m.shape != shape or not w.is_contiguous() or not m.is_contiguous():
-            raise KsrError(f"muon_update: tensor {i}: gradient and momentum must have the weight's shape {tuple(shape)}, weight "
-                           "and momentum be contiguous")
+    for shape, g, wp, mp in zip(shapes, grads, map(T.data_ptr, weights), map(T.data_ptr, momenta)):
         if len(shape) == 2:
             rows, cols = shape
             rs, cs = g.stride()
-        else:
+        elif len(shape) > 2:
             rows, cols = as_matrix(shape)
             g, rs, cs = g.contiguous(), cols, 1
             held.append(g)
+        else:
+            raise KsrError(f"muon_update: a tensor is {tuple(shape)}: matrices only (vectors belong to Adam)")
         if rows > 1 << 24 or cols > 1 << 24:
-            raise KsrError(f"muon_update: tensor {i}: {tuple(shape)} is too large")
-        wp, gp, mp = w.data_ptr(), g.data_ptr(), m.data_ptr()
+            raise KsrError(f"muon_update: a tensor is {tuple(shape)}: too large")
+        gp = g.data_ptr()
         if wp:
             nbytes = 4 * rows * cols
-            spans.append((wp, wp + nbytes))
-            spans.append((mp, mp + nbytes))
-            if gp == wp or gp == mp:
-                raise KsrError(f"muon_update: tensor {i}'s gradient is its weight or momentum")
+            spans += (wp, wp + nbytes, True), (mp, mp + nbytes, True), (gp, gp + 4 * ((rows - 1) * rs + (cols - 1) * cs + 1), False)
         words += gp, wp, mp, rs, cs, 0, rows | cols << 32, 1                # _matrix(...)
     spans.sort()
-    end = 0
-    for first, last in spans:                                   # the matrices of a call run side by side
-        if first < end:
-            raise KsrError("muon_update: weights or momenta of the list overlap, or one is in it twice")
-        end = last
+    written = read = 0                                          # where what is written, and read, so far ends
+    for first, last, write in spans:                            # the matrices of a call run side by side
+        if first < written or write and first < read:
+            raise KsrError("muon_update: weights or momenta of the list overlap each other or a gradient, or one is in it twice")
+        if write:
+            written = last
+        elif last > read:
+            read = last
     _run(words, weights[0], False, _split(precision, f32), steps, coefficients, eps, True, momentum, nesterov, grad_scale, lr,
          lr_dev, weight_decay, scale)
     # the kernels write behind torch's back: whoever keys on the version counters (autograd, the UNet's kernel-layout weights) sees it

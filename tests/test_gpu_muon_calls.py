@@ -96,3 +96,27 @@ def test_forward_mode_and_traced_updates_are_refused_not_dropped():
     with pytest.raises(KsrError, match="traced"):
         torch.jit.trace(update, (b,))
     assert all(torch.equal(t, u) for t, u in zip((a, b, c), before))
+
+
+def test_gradients_that_overlap_what_is_written_are_refused():
+    """The matrices of a call run side by side: one's weight may be written while another still reads it as its gradient."""
+    from kan_sr._lib import KsrError
+    from kan_sr.muon import muon_update
+    a, b, m, n = (randn(8, 8, seed=k) for k in range(4))
+    buf = randn(200, seed=9)
+    w, far = buf[8:72].view(8, 8), buf[120:184].view(8, 8)
+    before = [t.clone() for t in (a, b, m, n, buf)]
+    for ws, gs, ms in (([a, b], [b, a], [m, n]),                                   # crossed
+                       ([a, b], [randn(8, 8), m], [m, n]),                         # another entry's momentum
+                       ([w], [buf[0:64].view(8, 8)], [m]), ([w], [buf[71:135].view(8, 8)], [m]),        # partly its own weight
+                       ([a], [buf[60:124].view(8, 8)], [far]),                     # partly its own momentum
+                       ([w], [buf[:160:20].expand(8, 8)], [m]), ([w], [buf[:64].view(8, 8).t()], [m]),  # by its strides
+                       ([buf[8:72].view(4, 16)], [buf[72:136].view(4, 16)], [buf[135:199].view(4, 16)])):
+        with pytest.raises(KsrError, match="overlap"):
+            muon_update(ws, gs, ms, lr=0.1)
+    assert all(torch.equal(t, u) for t, u in zip((a, b, m, n, buf), before))
+    # neighbours in one buffer, and gradients that share memory, are fine
+    g = randn(8, 8, seed=10)
+    muon_update([w], [buf[72:136].view(8, 8)], [buf[136:200].view(8, 8)], lr=0.1)
+    muon_update([a, b], [g, g.t()], [m, n], lr=0.1)
+    muon_update([b], [g[:1].expand(8, 8)], [n], lr=0.1)
