@@ -739,11 +739,14 @@ class _UNetFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dw):
         want_gx = ctx.needs_input_grad[0]
+        sink = ctx.net.grad_sink is not None
+        if not sink and ctx.leaves != len(ctx.names):
+            raise KsrError("UNet: this forward was recorded with a grad_sink that is gone: its gradients have nowhere to go")
         grads = ctx.net._backward(ctx.tape, dw.contiguous(), want_input_grad=want_gx)
         ctx.tape = None
         gx = None
         if want_gx:         # [B,H,W,1] is [B,1,H,W]
             gx, ctx.net._input_grad = ctx.net._input_grad.view(-1, 1, *ctx.net._input_grad.shape[1:3]), None
-        if ctx.net.grad_sink is not None or ctx.leaves != len(ctx.names):
+        if sink:
             return (gx,) + (None,) * (3 + ctx.leaves)
         return (gx, None, None, None) + tuple(grads[n].contiguous() for n in ctx.names)
