@@ -1,4 +1,4 @@
-"""Group norm + activation (kan_sr.ops.group_norm_act) in calls of the largest numbers of groups, traces and forward mode."""
+"""Group norm + activation (kan_sr.ops.group_norm_act) in calls of the largest numbers of groups, traces, forward mode, streams."""
 import pytest
 import torch
 
@@ -92,3 +92,38 @@ def test_relu_has_one_mask(shape, G, dtype):
     assert float((y.detach().float().reshape(-1, C)[(x.detach() == level.to(dtype).cuda()).reshape(-1, C).any(dim=1)]).min()) == 0.0
     db, = torch.autograd.grad(y, (b,), torch.ones_like(y))
     assert torch.equal(db, (y > 0).reshape(-1, C).sum(dim=0).float())
+
+
+def test_calls_that_overlap_on_three_streams():
+    """Forward and backward of several hundred microseconds each, queued behind one event and then let go together: a workspace that
+    two calls shared would mix their sums."""
+    from kan_sr.ops import group_norm_act
+    args = []
+    for k, (shape, G, dtype) in enumerate([((3, 256, 256, 320), 32, torch.bfloat16), ((4, 300, 300, 90), 9, torch.float32),
+                                           ((24, 128, 128, 256), 32, torch.float32)]):
+        g = torch.Generator("cuda").manual_seed(k)
+        x, dy = ((torch.randn(shape, device="cuda", generator=g) + k).to(dtype) for _ in range(2))
+        w, b = (torch.randn(shape[-1], device="cuda", generator=g) for _ in range(2))
+        args.append((x.requires_grad_(), w.requires_grad_(), b.requires_grad_(), dy, G))
+
+    def run(x, w, b, dy, G):
+        y = group_norm_act(x, G, w, b, activation="silu")
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy)
+
+    want = [run(*a) for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    gate, go = torch.randn(8192, 8192, device="cuda"), torch.cuda.Event()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):                                  # about 50 ms, while the calls are queued
+        gate = gate @ gate * 1e-2
+    go.record()
+    for st in streams:
+        st.wait_event(go)
+    for k in range(4):
+        for a, st in zip(args, streams):
+            with torch.cuda.stream(st):
+                got.append(run(*a))
+    torch.cuda.synchronize()
+    for k, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[k % 3])), k
