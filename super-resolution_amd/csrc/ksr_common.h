@@ -20,12 +20,6 @@ const unsigned long long* ksr_seed_dev();
         if ((a).seed_dev) (a).seed += *(a).seed_dev * 0x9E3779B97F4A7C15ULL;   \
     } while (0)
 
-// activations of the group norm (include/ksr.h)
-#define KSR_ACT_NONE 0
-#define KSR_ACT_RELU 1
-#define KSR_ACT_SILU 2
-#define KSR_ACT_GELU 3
-
 #define KSR_MAX_KNOTS 64
 #define KSR_MAX_ORDER 3
 

@@ -1,5 +1,6 @@
 // What the group norm's kernels share (ksr_group_norm.hip: chunks of an image; ksr_group_norm_one.hip: a group in registers).
 #pragma once
+#include "ksr.h"
 #include "ksr_common.h"
 
 struct GnArgs {
