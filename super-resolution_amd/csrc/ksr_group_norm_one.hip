@@ -229,7 +229,9 @@ __global__ void __launch_bounds__(TH) gn_one_bwd_kernel(GnArgs a) {
     }
 }
 
-// bytes a thread holds of each tensor: at most 40 (20) vectors of them, less where the statistics of four groups or more need room
+// bytes a thread holds of each tensor: at most 40 (20) vectors of them, less where the statistics of four groups or more need room.
+// Of the workgroups of 1024 threads (128 registers each) the bf16 ones in vectors of 8 still spill: forward with eight groups a
+// vector (one channel each) 150 registers, backward 4 to 41 by activation and groups; the others none.
 constexpr int hold(bool bwd, int bytes, int ne) { return bwd ? (bytes < 8 ? 20 * bytes : 128) : (bytes < 8 ? 40 * bytes : ne >= 4 ? 128 : 256); }
 
 template <class T, int VEC, int NE, int TH, int HOLD, bool BWD> int launch(const GnArgs& a, int act, hipStream_t st) {

@@ -127,7 +127,8 @@ __device__ __forceinline__ double wave_sum(double v) {
 // slabs of 32 columns in the accumulator layout of v_mfma_f32_32x32x16 (lane = column, register r = row 8 (r/4) + 4 (lane/32) +
 // r%4), which is the B operand's layout for the next product when both operands take k in that order.  Always SPLIT: the time
 // is latency (one wave or two per SIMD, three or four barriers a step), not matrix work.  fp32, five steps: 26 us for 64 x 64, 97 us
-// for 1 or 16 of 64 x 1024; as large matrices 245 to 265 us, in 17 launches.
+// for 1 or 16 of 64 x 1024; as large matrices 245 to 265 us, in 17 launches.  Four slabs (513 columns and more) do not fit 256
+// registers: 34 (Muon 110, bf16 26) are spilled.
 // The 64 x 64 matrices A and A^2 are four 32 x 32 tiles of four waves; both triangles are computed, so that a wave writes its
 // tile's transpose in 8-byte pieces and nothing else (symmetric up to the rounding of hi lo + lo hi).  For X X^T the slabs pass
 // through LDS, eight at a time, the upper four waves taking slabs 4 to 7 of them.

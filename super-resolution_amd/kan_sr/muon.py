@@ -60,8 +60,10 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
     """Orthogonalises the matrices g [..., rows, cols] (float32 or bfloat16, any strides): a dense tensor of g's shape and type.
 
     X = g / (|g|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (of the transposed matrix where
-    rows > cols).  precision: "fp32" (default for float32) forms the products to fp32 accuracy, "bf16" (default for bfloat16) to
-    that of a bfloat16 result at a third of the matrix work.  Not differentiable."""
+    rows > cols).  precision: "fp32" (default for float32) forms the products to fp32 accuracy (operands of 22 bits); "bf16"
+    (default for bfloat16) takes a third of the matrix work with operands of 11 bits: 2e-4 to 9e-4 of the result before it is
+    rounded to bfloat16, which is 1.7e-3 by itself; pass "fp32" where bfloat16 results have to be those of fp32 products.  A
+    matrix's result does not depend on what else is in the call.  Not differentiable."""
     steps, coefficients = _steps_and_coefficients(steps, coefficients)
     if g.dim() < 2:
         raise KsrError(f"newton_schulz: g must be [..., rows, cols], got {tuple(g.shape)}")
