@@ -225,7 +225,7 @@ def _address(t: Optional[torch.Tensor]):
 
 
 def _group_norm_fwd(x, weight, bias, groups, eps, act):
-    """-> (y, x as it was read, statistics, (image stride, pixel stride, pixels))."""
+    """-> (y, x as it was read, statistics)."""
     x, xb, xp, S = _pixel_rows(x)
     B, C = x.shape[0], x.shape[-1]
     L = lib()
@@ -238,22 +238,23 @@ def _group_norm_fwd(x, weight, bias, groups, eps, act):
         ws = torch.empty(n, device=x.device, dtype=torch.float32)
         check(L.ksr_group_norm_fwd(x.data_ptr(), xb, xp, _address(weight), _address(bias), y.data_ptr(), stats.data_ptr(),
                                    ws.data_ptr(), B, S, C, groups, eps, act, x.dtype is torch.bfloat16, stream()), "ksr_group_norm_fwd")
-    return y, x, stats, (xb, xp, S)
+    return y, x, stats
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, x, stats, layout = _group_norm_fwd(x, weight, bias, groups, eps, act)
+        y, x, stats = _group_norm_fwd(x, weight, bias, groups, eps, act)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.cfg = (groups, act) + layout
+        ctx.cfg = (groups, act)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
-        groups, act, xb, xp, S = ctx.cfg
+        groups, act = ctx.cfg
+        x, xb, xp, S = _pixel_rows(x)          # as it is now: saved-tensor hooks (save_on_cpu) bring it back dense
         B, C = x.shape[0], x.shape[-1]
         dy, gb, gp, _ = _pixel_rows(dy)
         want_x, want_w, want_b = ctx.needs_input_grad[:3]

@@ -127,3 +127,22 @@ def test_calls_that_overlap_on_three_streams():
     torch.cuda.synchronize()
     for k, out in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(out, want[k % 3])), k
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensors_that_come_back_with_other_strides(dtype):
+    """save_on_cpu stores a channel slice densely: its strides of the forward would reach beyond it in the backward."""
+    from kan_sr.ops import group_norm_act
+    big = torch.randn(2, 30, 20, 64, device="cuda").to(dtype)
+    dy = torch.randn(2, 30, 20, 24, device="cuda").to(dtype)
+    w, b = torch.randn(24, device="cuda", requires_grad=True), torch.randn(24, device="cuda", requires_grad=True)
+    for x in (big[..., 8:32], big[..., 3:27], big[:1, :1, :1, :24].expand(2, 30, 20, 24)):
+        x = x.detach().requires_grad_()
+        want = torch.autograd.grad(group_norm_act(x, 4, w, b, activation="gelu"), (x, w, b), dy)
+        with torch.autograd.graph.save_on_cpu():
+            y = group_norm_act(x, 4, w, b, activation="gelu")
+        for p, q in zip(torch.autograd.grad(y, (x, w, b), dy), want):
+            # other vectors, another order of the sums: at most 64 roundings of each of two terms of the largest gradient's size; a
+            # bfloat16 result may end one step away
+            tol = 128 * U32 * q.abs().max() + (torch.finfo(dtype).eps * q.abs() if q.dtype is torch.bfloat16 else 0)
+            assert bool(((p - q).abs() <= tol).all())
