@@ -180,7 +180,10 @@ def muon_update(weights, grads, momenta, lr: float, momentum: float = 0.95, nest
     _run(words, weights[0], False, _split(precision, f32), steps, coefficients, eps, True, momentum, nesterov, grad_scale, lr,
          lr_dev, weight_decay, scale)
     # the kernels write behind torch's back: whoever keys on the version counters (autograd, the UNet's kernel-layout weights) sees it
-    torch.autograd.graph.increment_version(weights + momenta)
+    try:
+        torch.autograd.graph.increment_version(weights + momenta)
+    except RuntimeError:                             # tensors made in inference mode have no counter, the others still need theirs
+        torch.autograd.graph.increment_version([t for t in weights + momenta if not t.is_inference()])
 
 
 class Muon(torch.optim.Optimizer):

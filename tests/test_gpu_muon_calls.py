@@ -120,3 +120,19 @@ def test_gradients_that_overlap_what_is_written_are_refused():
     muon_update([w], [buf[72:136].view(8, 8)], [buf[136:200].view(8, 8)], lr=0.1)
     muon_update([a, b], [g, g.t()], [m, n], lr=0.1)
     muon_update([b], [g[:1].expand(8, 8)], [n], lr=0.1)
+
+
+def test_tensors_made_in_inference_mode():
+    """They have no version counter to bump: the update of all, and the counters of the others, are as ever."""
+    from kan_sr.muon import muon_update
+    g = [1e-3 * randn(24, 40, seed=2), 1e-3 * randn(70, 30, seed=3)]
+    with torch.inference_mode():
+        w = [randn(24, 40)]
+    w.append(randn(70, 30))
+    m = [torch.zeros(24, 40, device="cuda"), torch.zeros(70, 30, device="cuda")]
+    copies = [t.clone() for t in w], [t.clone() for t in m]
+    before = [t._version for t in (w[1], *m)]
+    muon_update(w, g, m, lr=0.1)
+    assert all(t._version > v for t, v in zip((w[1], *m), before))
+    muon_update(copies[0], g, copies[1], lr=0.1)
+    assert all(torch.equal(a, b) for a, b in zip(w + m, copies[0] + copies[1]))
