@@ -670,8 +670,9 @@ __global__ void __launch_bounds__(256) ns_prepare_kernel(LargeArgs a) {
 // that read at once hit all banks.
 // Sums: along k in chunks of `chunk_of` columns; a chunk's sum is added to the tile's in the order of k.  Shorter chains of
 // roundings, and the result does not depend on who computes which chunk.  X of single operands has one chain instead (the
-// 256 x 256 tile has no registers for a second sum) and is never cut, so that a tile of any size gives the same bits (bf16 against
-// chains and cuts that followed the tile: 2100 x 2100 602 us for 554, 2560 x 2560 723 for 864, 1536 x 1536 339 for 369).
+// 256 x 256 tile has no registers for a second sum) and is never cut, so that a tile of any size gives the same bits.  bf16 squares,
+// against chains and cuts that followed the tile: 1536 339 us for 369, 1792 424 for 599, 2560 723 for 864, but 2100 579 for 534
+// and 2944 1027 for 938, whose 128 x 128 tiles just pass a multiple of the workgroups that run at once.
 // Work split: of T tiles the first `whole` = 256 floor(T / 256) have a workgroup each; each chunk of the others has one of its
 // own (`cut`), so that a round that is not full still occupies the chip (528 tiles would otherwise take as long as 768).  Such a
 // workgroup leaves its fp32 sums in the workspace; the one that arrives last adds them in order and goes on with the tile.
