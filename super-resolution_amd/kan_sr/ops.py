@@ -195,7 +195,8 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}          # KSR_ACT_* 
 def _pixel_rows(t: torch.Tensor):
     """t [B, ..., C] -> (t or a dense copy, image stride, pixel stride, pixels): in place where the channels are contiguous
     and the middle dimensions are one run of pixels (dense tensors, channel slices, images of a larger buffer)."""
-    B, C, n = t.shape[0], t.shape[-1], t.numel()
+    shape, n = t.shape, t.numel()
+    B, C = shape[0], shape[-1]
     if n and t.is_contiguous():
         S = n // (B * C)
         return t, S * C if B > 1 else 0, C if S > 1 else 0, S
@@ -255,18 +256,19 @@ class _GroupNormAct(torch.autograd.Function):
         x, weight, bias, stats = ctx.saved_tensors
         groups, act = ctx.cfg
         x, xb, xp, S = _pixel_rows(x)          # as it is now: saved-tensor hooks (save_on_cpu) bring it back dense
-        B, C = x.shape[0], x.shape[-1]
+        shape, dtype, device = x.shape, x.dtype, x.device
+        B, C = shape[0], shape[-1]
         dy, gb, gp, _ = _pixel_rows(dy)
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         L = lib()
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_x else None
-        dw = torch.empty(C, device=x.device, dtype=torch.float32) if want_w else None
-        db = torch.empty(C, device=x.device, dtype=torch.float32) if want_b else None
+        dx = torch.empty(shape, device=device, dtype=dtype) if want_x else None
+        dw = torch.empty(C, device=device, dtype=torch.float32) if want_w else None
+        db = torch.empty(C, device=device, dtype=torch.float32) if want_b else None
         with on_device_of(x):
-            ws = torch.empty(L.ksr_group_norm_ws_floats(B, S, C, groups, 1), device=x.device, dtype=torch.float32)
+            ws = torch.empty(L.ksr_group_norm_ws_floats(B, S, C, groups, 1), device=device, dtype=torch.float32)
             check(L.ksr_group_norm_bwd(x.data_ptr(), xb, xp, dy.data_ptr(), gb, gp, _address(weight), _address(bias), stats.data_ptr(),
                                        _address(dx), _address(dw), _address(db), ws.data_ptr(), B, S, C, groups, act,
-                                       x.dtype is torch.bfloat16, stream()), "ksr_group_norm_bwd")
+                                       dtype is torch.bfloat16, stream()), "ksr_group_norm_bwd")
         return dx, dw, db, None, None, None
 
 
